@@ -331,11 +331,56 @@ typedef struct mattn_row_copy {
  * dimension, and the columns of padded gradients taken back. */
 int mattn_copy_rows(const mattn_row_copy* copies, int32_t n, void* stream);
 
+/*
+ * Rotary positions of one or two tensors (queries and keys) [B, L, H[t], D], with or
+ * without the RMS norm of each head's row before them:
+ *
+ *   y = x (norm = 0), or x r w with r = (mean(x^2) + eps)^-1/2 (norm = 1)
+ *   z = y with the pairs of its first `dim` columns turned by the angle
+ *       p * inv_freq[i] (by its negative where inverse = 1) and scaled by `scale`;
+ *       pair i is the columns (i, i + dim / 2) or (2 i, 2 i + 1)
+ *
+ * p is the position of (b, l): l itself (pos_bytes = 0) or positions[b * pos_stride[0]
+ * + l * pos_stride[1]], 4 or 8 byte integers.  Angles are formed in float64, statistics
+ * in float32; z has x's dtype, rounded once.  D <= 512; the D columns are contiguous,
+ * rows may have any alignment (16-byte accesses where all strides, addresses, dim / 2
+ * and D - dim are multiples of 16 bytes).  z must not overlap its inputs.  The gradient
+ * of the rotation is the call with inverse flipped; the norm's is mattn_norm_rotary_bwd.
+ */
+enum mattn_rotary_layout { MATTN_ROTARY_HALF = 0, MATTN_ROTARY_INTERLEAVED = 1 };
+typedef struct mattn_rotary {
+  int32_t B, L, D, dim;
+  int32_t n;                   /* tensors: 1 or 2                                    */
+  int32_t H[2];
+  int32_t dtype;               /* enum mattn_dtype of x, y, g                        */
+  int32_t layout;              /* enum mattn_rotary_layout                           */
+  int32_t inverse, norm;
+  int32_t pos_bytes;           /* 0 (positions 0 .. L - 1), 4 or 8                    */
+  float eps, scale;
+  int64_t pos_stride[2];       /* in elements                                        */
+  int64_t x_stride[2][3], y_stride[2][3], g_stride[2][3];   /* {batch, sequence, head} */
+  const void* x[2];            /* inputs                                             */
+  void* y[2];                  /* outputs (backward: the gradients of x)             */
+  const void* g[2];            /* backward: the gradients of z (forward: unused)     */
+  const float* w[2];           /* norm: weights [D] float32, NULL for ones           */
+  const void* positions;
+  const double* inv_freq;      /* [dim / 2]                                          */
+} mattn_rotary;
+
+int mattn_rotary_fwd(const mattn_rotary* p, void* stream);
+
+/* Gradients of the call with norm = 1: y[t] = the gradients of x[t], dw0 and dw1 [D]
+ * float32 those of the weights (both NULL: not formed).  The workspace holds partial
+ * sums, which are added in a fixed order. */
+size_t mattn_norm_rotary_bwd_workspace_bytes(const mattn_rotary* p);
+int mattn_norm_rotary_bwd(const mattn_rotary* p, float* dw0, float* dw1, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 /* Static text of a status code. */
 const char* mattn_strerror(int status);
 
 /* Library ABI version (bumped on any change of the structs, flags or functions above;
- * 9: MATTN_DO_16 and mattn_copy_rows). */
+ * 10: rotary positions). */
 int mattn_abi_version(void);
 
 #ifdef __cplusplus

@@ -21,7 +21,7 @@ MATTN_BWD_DS = 2
 MATTN_PRECISE = 4
 MATTN_DO_16 = 16
 TILE_Q = TILE_K = 128
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 STATUS = {
     0: "MATTN_OK",
@@ -43,7 +43,8 @@ STATUS = {
 EXPORTS = ("mattn_validate", "mattn_workspace_bytes", "mattn_bwd_workspace_bytes", "mattn_fwd_workspace_bytes",
            "mattn_fwd", "mattn_bwd",
            "mattn_bwd_stage", "mattn_strerror", "mattn_abi_version", "mattn_maskspec_validate",
-           "mattn_tilemap_classify", "mattn_tilemap_bits", "mattn_bwd_noalloc", "mattn_copy_rows")
+           "mattn_tilemap_classify", "mattn_tilemap_bits", "mattn_bwd_noalloc", "mattn_copy_rows",
+           "mattn_rotary_fwd", "mattn_norm_rotary_bwd_workspace_bytes", "mattn_norm_rotary_bwd")
 SCRATCH_BYTES = 512 << 20  # MATTN_SCRATCH_BYTES
 BWD_PRE, BWD_DKDV, BWD_DQ = 0, 1, 2
 
@@ -91,6 +92,22 @@ class MattnRowCopy(ctypes.Structure):
         ("src_stride", _I64x3), ("dst_stride", _I64x3), ("n", ctypes.c_int32 * 3),
         ("src_dtype", ctypes.c_int32), ("dst_dtype", ctypes.c_int32),
         ("src_cols", ctypes.c_int32), ("dst_cols", ctypes.c_int32),
+    ]
+
+
+_I64x2 = ctypes.c_int64 * 2
+_PTRx2 = ctypes.c_void_p * 2
+
+
+class MattnRotary(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("D", ctypes.c_int32), ("dim", ctypes.c_int32),
+        ("n", ctypes.c_int32), ("H", ctypes.c_int32 * 2), ("dtype", ctypes.c_int32), ("layout", ctypes.c_int32),
+        ("inverse", ctypes.c_int32), ("norm", ctypes.c_int32), ("pos_bytes", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("scale", ctypes.c_float), ("pos_stride", _I64x2),
+        ("x_stride", _I64x3 * 2), ("y_stride", _I64x3 * 2), ("g_stride", _I64x3 * 2),
+        ("x", _PTRx2), ("y", _PTRx2), ("g", _PTRx2), ("w", _PTRx2),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
     ]
 
 
@@ -150,6 +167,13 @@ def load():
         lib.mattn_tilemap_bits.restype = ctypes.c_int
         lib.mattn_copy_rows.argtypes = [ctypes.POINTER(MattnRowCopy), i32, vp]
         lib.mattn_copy_rows.restype = ctypes.c_int
+        R = ctypes.POINTER(MattnRotary)
+        lib.mattn_rotary_fwd.argtypes = [R, vp]
+        lib.mattn_rotary_fwd.restype = ctypes.c_int
+        lib.mattn_norm_rotary_bwd_workspace_bytes.argtypes = [R]
+        lib.mattn_norm_rotary_bwd_workspace_bytes.restype = ctypes.c_size_t
+        lib.mattn_norm_rotary_bwd.argtypes = [R, vp, vp, vp, sz, vp]
+        lib.mattn_norm_rotary_bwd.restype = ctypes.c_int
         lib.mattn_abi_version.argtypes = []
         lib.mattn_abi_version.restype = ctypes.c_int
         if lib.mattn_abi_version() != ABI_VERSION:

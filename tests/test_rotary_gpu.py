@@ -1,0 +1,253 @@
+"""Rotary positions and head norms (GPU) against float64 on the CPU.
+
+Tolerances.  A result of a 16-bit dtype is off by half a step, eps / 2 of its value (and
+half the smallest subnormal).  Before that rounding everything is float32: u = 2^-24 of
+the sum of the terms' magnitudes for each operation of a chain.  A turned column is two
+products and a sum of values whose cosines and sines are off by 4 u (an angle reduced in
+float64, rounded once, and the function's own error): 8 u.  The norm adds a sum of D
+squares (at most D / 2 in one chain of additions, each u; half of that through the root),
+the root, the division and two products: D / 4 + 8.  The gradient adds the mean of D
+products of such terms: in all below D + 32.  A weight's gradient adds the rows of one
+thread and of the joining steps: below rows / 8192 + 128 terms in one chain.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import rotary_oracle as ro
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _close(got, want, mag, units, what):
+    dt = got.dtype
+    got = got.detach().double().cpu().numpy()
+    tol = units * U * mag
+    if dt != torch.float32:
+        tol = tol + torch.finfo(dt).eps / 2 * np.abs(want) * (1 + units * U) + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float(np.nanmax(np.abs(got - want) / np.maximum(tol, 1e-300))))
+
+
+def _freq(pairs, **kw):
+    import jaxmodules_amd as jm
+
+    return jm.rotary_frequencies(2 * pairs, device="cuda", **kw)
+
+
+def _pair(B, L, Hq, Hk, D, dtype, seed, f=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return [(torch.randn((B, L, H, D), generator=gen, device="cuda") * f).to(getattr(torch, dtype)) for H in (Hq, Hk)]
+
+
+SHAPES = [
+    # B, L, Hq, Hk, D, dim
+    (1, 1, 1, 1, 2, 2), (2, 1, 8, 2, 64, 64), (1, 130, 4, 4, 128, 128), (3, 37, 5, 1, 128, 64), (2, 9, 3, 2, 96, 96),
+    (1, 700, 32, 8, 64, 64), (2, 17, 2, 1, 80, 40), (1, 5, 2, 2, 127, 62), (1, 6, 3, 1, 512, 512), (1, 3, 2, 2, 511, 254),
+    (70, 1, 3, 1, 256, 128), (1, 4099, 2, 1, 32, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rotary(shape, layout, dtype):
+    import jaxmodules_amd as jm
+
+    B, L, Hq, Hk, D, dim = shape
+    q, k = _pair(B, L, Hq, Hk, D, dtype, L + D)
+    g = _pair(B, L, Hq, Hk, D, dtype, L + D + 1)
+    f, scale = _freq(dim // 2, scaling="parts" if dim > 16 else None, factor=8.0, context=4096)
+    pos = torch.randint(-100, 1 << 20, (B, L), device="cuda", generator=torch.Generator(device="cuda").manual_seed(D))
+    q, k = q.requires_grad_(), k.requires_grad_()
+    out = jm.rotary(q, k, pos, inv_freq=f, layout=layout, scale=scale)
+    grads = torch.autograd.grad(out, (q, k), g)
+    p, w = pos.cpu().numpy(), f.cpu().numpy()
+    for x, y, u, dx in zip((q, k), out, g, grads):
+        assert y.dtype == x.dtype and y.is_contiguous()
+        _close(y, *ro.turn(x.detach().double().cpu().numpy(), p, w, layout, scale), 8, "z")
+        _close(dx, *ro.turn(u.double().cpu().numpy(), p, w, layout, scale, -1.0), 8, "dx")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_norm_rotary(shape, layout, dtype):
+    import jaxmodules_amd as jm
+
+    B, L, Hq, Hk, D, dim = shape
+    q, k = (x.requires_grad_() for x in _pair(B, L, Hq, Hk, D, dtype, L + D))
+    g = _pair(B, L, Hq, Hk, D, dtype, L + D + 1)
+    wq, wk = ((torch.randn(D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)) * 0.3 + 1).requires_grad_()
+              for i in range(2))
+    f, scale = _freq(dim // 2)
+    eps = 1e-5
+    out = jm.norm_rotary(q, k, wq, wk, inv_freq=f, layout=layout, scale=scale, eps=eps)
+    grads = torch.autograd.grad(out, (q, k, wq, wk), g)
+    p, fr = np.broadcast_to(np.arange(L), (B, L)), f.cpu().numpy()
+    for i, (x, w, y, u) in enumerate(zip((q, k), (wq, wk), out, g)):
+        X, W, G = (t.detach().double().cpu().numpy() for t in (x, w, u))
+        _close(y, *ro.norm_turn(X, W, p, fr, layout, scale, eps), D / 4 + 16, "z")
+        (dx, mx), (dw, mw) = ro.norm_turn_grads(X, W, G, p, fr, layout, scale, eps)
+        _close(grads[i], dx, mx, D + 32, "dx")
+        _close(grads[2 + i], dw, mw, D + 32 + B * L * x.shape[2] / 8192 + 128, "dw")
+
+
+def test_weights_of_the_inputs_dtype_and_none():
+    import jaxmodules_amd as jm
+
+    q, k = (x.requires_grad_() for x in _pair(2, 33, 4, 2, 64, "bfloat16", 3))
+    w = (torch.randn(64, device="cuda") + 1).bfloat16().requires_grad_()
+    f, _ = _freq(32)
+    a = jm.norm_rotary(q, k, w, None, inv_freq=f)
+    b = jm.norm_rotary(q, k, w.detach().float(), torch.ones(64, device="cuda"), inv_freq=f)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    dw, = torch.autograd.grad(a, w, [torch.ones_like(x) for x in a])
+    assert dw.dtype == torch.bfloat16
+    n = jm.norm_rotary(q.detach(), k.detach(), w.detach())  # the norm alone
+    X = q.detach().double().cpu().numpy()
+    want = ro.norm(X, None, 1e-6)[0] * w.detach().double().cpu().numpy()
+    _close(n[0], want, np.abs(want), 64 / 4 + 16, "norm")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D,dim", [(64, 64), (128, 64)])
+def test_strides(dtype, D, dim):
+    """Slices of a fused projection, heads before positions, odd addresses, expanded
+    gradients: bitwise what dense copies give."""
+    import jaxmodules_amd as jm
+
+    dt = getattr(torch, dtype)
+    B, L, H = 2, 21, 3
+    f, _ = _freq(dim // 2)
+    w = torch.rand(D, device="cuda") + 0.5
+    fused = torch.randn(B, L, 3 * H * D + 8, device="cuda").to(dt)
+    flat = torch.randn(B * L * H * D + 1, device="cuda").to(dt)
+    views = [fused[:, :, : H * D].view(B, L, H, D), fused[:, :, H * D + 1: 2 * H * D + 1].unflatten(2, (H, D)),
+             torch.randn(B, H, L, D, device="cuda").to(dt).transpose(1, 2), flat[1:].view(B, L, H, D),
+             torch.randn(B, L, H, 2 * D, device="cuda").to(dt)[..., ::2], torch.randn(1, L, 1, D, device="cuda").to(dt).expand(B, L, H, D)]
+    for v in views:
+        for fn in (lambda x: jm.rotary(x, inv_freq=f), lambda x: jm.norm_rotary(x, None, w, inv_freq=f)):
+            x, c = v.detach().requires_grad_(), v.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
+            a, b = fn(x), fn(c)
+            # (16-byte and single accesses add the norm's squares in other orders)
+            tol = dict(rtol=2 ** -6 if dt == torch.bfloat16 else 2 ** -19, atol=2 ** -20)
+            torch.testing.assert_close(a, b, **tol)
+            g = torch.randn(1, 1, 1, D, device="cuda").to(dt).expand(B, L, H, D)
+            torch.testing.assert_close(torch.autograd.grad(a, x, g)[0], torch.autograd.grad(b, c, g.contiguous())[0],
+                                       rtol=tol["rtol"], atol=2 ** -8 if dt == torch.bfloat16 else 2 ** -16)
+
+
+def test_positions_and_three_dimensions():
+    import jaxmodules_amd as jm
+
+    q, k = _pair(1, 12, 2, 1, 64, "float32", 5)
+    f, _ = _freq(32)
+    base = jm.rotary(q, k, inv_freq=f)
+    for pos in (torch.arange(12), torch.arange(12, dtype=torch.int32), torch.arange(24)[::2] // 2, torch.arange(12)[None]):
+        assert all(torch.equal(a, b) for a, b in zip(base, jm.rotary(q, k, pos.cuda(), inv_freq=f)))
+    three = jm.rotary(q[0], k[0], inv_freq=f)
+    assert all(torch.equal(a[0], b) for a, b in zip(base, three))
+    assert torch.equal(jm.rotary(q, inv_freq=f), base[0])
+
+
+def test_empty():
+    import jaxmodules_amd as jm
+
+    f, _ = _freq(32)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for shape in ((0, 4, 2, 64), (2, 0, 2, 64)):
+        q = torch.zeros(shape, device="cuda", requires_grad=True)
+        assert jm.rotary(q, inv_freq=f).shape == q.shape
+        o = jm.norm_rotary(q, None, w, inv_freq=f)
+        dq, dw = torch.autograd.grad(o, (q, w), torch.zeros_like(o))
+        assert dq.shape == q.shape and not dw.any()
+    q, k = torch.randn(1, 3, 2, 64, device="cuda"), torch.zeros(1, 3, 0, 64, device="cuda")
+    a, b = jm.norm_rotary(q, k, w.detach(), w.detach(), inv_freq=f)
+    assert torch.equal(a, jm.norm_rotary(q, None, w.detach(), inv_freq=f)) and b.shape == k.shape
+
+
+def test_other_values_stay_their_own():
+    """Infinities and NaN of one row reach no other row."""
+    import jaxmodules_amd as jm
+
+    q, _ = _pair(1, 40, 4, 1, 64, "bfloat16", 9)
+    f, _ = _freq(32)
+    clean = jm.norm_rotary(q, inv_freq=f)
+    bad = q.clone()
+    bad[0, 7, 2, 5], bad[0, 9, 0, 1] = float("nan"), float("inf")
+    out = jm.norm_rotary(bad, inv_freq=f)
+    same = torch.ones(1, 40, 4, dtype=torch.bool, device="cuda")
+    same[0, 7, 2] = same[0, 9, 0] = False
+    assert torch.equal(out[same], clean[same]) and out[0, 7, 2].isnan().all()
+
+
+def test_changed_weights_before_the_backward_are_an_error():
+    import jaxmodules_amd as jm
+
+    q = torch.randn(1, 3, 2, 64, device="cuda", requires_grad=True)
+    w, pos = torch.ones(64, device="cuda"), torch.arange(3, device="cuda")
+    f, _ = _freq(32)
+    for t in (w, pos):
+        o = jm.norm_rotary(q, None, w, positions=pos, inv_freq=f)
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.sum().backward()
+
+
+def test_gradient_against_differences():
+    """(f(x + h) - f(x - h)) / 2 of the entry point itself, in float32: h^2 of the third
+    derivative and u / h of the values, both below 1e-2 of the gradient's size here."""
+    import jaxmodules_amd as jm
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn((1, 3, 2, 64), generator=gen, device="cuda").requires_grad_()
+    w = torch.rand(64, generator=gen, device="cuda").requires_grad_()
+    f, _ = _freq(16)
+    u = torch.randn(q.shape, generator=gen, device="cuda")
+    loss = lambda a, b: (jm.norm_rotary(a, None, b, inv_freq=f, layout="interleaved").double() * u).sum()  # noqa: E731
+    dq, dw = torch.autograd.grad(loss(q, w), (q, w))
+    with torch.no_grad():
+        for _ in range(6):
+            a, b = torch.randn(q.shape, generator=gen, device="cuda"), torch.randn(w.shape, generator=gen, device="cuda")
+            h = 2.0 ** -7
+            num = (loss(q + h * a, w + h * b) - loss(q - h * a, w - h * b)) / (2 * h)
+            want = (dq.double() * a).sum() + (dw.double() * b).sum()
+            size = (dq.double() * a).norm() + (dw.double() * b).norm()
+            assert abs(num - want) <= 1e-2 * size
+
+
+def test_side_stream_and_graph():
+    """On a stream of its own, and captured: every replay equals the eager result."""
+    import jaxmodules_amd as jm
+
+    q, k = _pair(2, 50, 4, 2, 64, "bfloat16", 1)
+    g = _pair(2, 50, 4, 2, 64, "bfloat16", 2)
+    w = torch.rand(64, device="cuda")
+    f, _ = _freq(32)
+    pos = torch.arange(50, device="cuda")
+
+    def step():
+        leaves = [x.detach().requires_grad_() for x in (q, k, w)]
+        out = jm.norm_rotary(leaves[0], leaves[1], leaves[2], leaves[2], pos, inv_freq=f)
+        return [x.detach() for x in out] + list(torch.autograd.grad(out, leaves, g))
+
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(side, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        q.copy_(torch.randn_like(q))
+        pos.add_(1000)
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
