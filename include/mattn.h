@@ -376,11 +376,92 @@ size_t mattn_norm_rotary_bwd_workspace_bytes(const mattn_rotary* p);
 int mattn_norm_rotary_bwd(const mattn_rotary* p, float* dw0, float* dw1, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/*
+ * Mean of the keys of each block of block_size: means [B, ceil(L / block_size), H, D]
+ * float32 (dense), float64 sums rounded once, over the keys below lengths[b] (NULL: L;
+ * clamped to [0, L]); 0 where a block holds none.  new_keys > 0: only the blocks that
+ * hold one of the last new_keys keys of each sequence are written.  Any alignment
+ * (16-byte accesses where addresses, strides and D allow them).
+ */
+typedef struct mattn_means {
+  int32_t B, L, H, D;
+  int32_t dtype;               /* enum mattn_dtype of k */
+  int32_t block_size, new_keys;
+  int64_t k_stride[3];         /* elements: batch, sequence, head; D contiguous */
+  const void* k;
+  float* means;
+  const int32_t* lengths;      /* [B] or NULL */
+} mattn_means;
+
+int mattn_block_means(const mattn_means* p, void* stream);
+
+/*
+ * Blocks for each query and key head: blocks [B, L, Hkv, count] int32 (dense), ascending,
+ * -1 behind.  Query q of sequence b is at position starts[b] + q (NULL: q).  It sees the
+ * blocks below ceil(lengths[b] / block_size) (NULL: nblk) and, causal, up to its own
+ * position's.  Of those the `first` first and `last` last are taken, then the best of the
+ * others by the score (sum over the group's heads of q) . mean in float64, ties to the
+ * lower index, NaN lowest.  D % 8 == 0, D <= 256; 16-byte aligned rows.
+ */
+typedef struct mattn_select {
+  int32_t B, L, nblk, Hq, Hkv, D;
+  int32_t dtype;               /* enum mattn_dtype of q */
+  int32_t block_size, count, first, last, causal;
+  int64_t q_stride[3];
+  int64_t m_stride[3];         /* of the means: batch, block, head */
+  const void* q;
+  const float* means;
+  const int32_t* starts;       /* [B] or NULL */
+  const int32_t* lengths;      /* [B] or NULL */
+  int32_t* blocks;
+} mattn_select;
+
+size_t mattn_select_workspace_bytes(const mattn_select* p);
+int mattn_select_blocks(const mattn_select* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Softmax attention of each query over the keys of its blocks.  blocks is
+ * [B, Lq, Hkv, count] int32, dense; entries outside the blocks a query sees and repeated
+ * ones are skipped.  Query q of sequence b is at position starts[b] + q (NULL: q) and
+ * sees keys below lengths[b] (NULL: Lk; clamped to [0, Lk]) and, causal, up to its own
+ * position.  A query without a key gives zeros.  D % 8 == 0, D <= 128, block_size a
+ * multiple of 16, count <= 1024; 16-byte aligned rows; o, dq, dk and dv have q's dtype.
+ */
+typedef struct mattn_selected {
+  int32_t B, Lq, Lk, Hq, Hkv, D;
+  int32_t dtype;
+  int32_t block_size, count, causal;
+  float scale;                 /* of the scores; finite */
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  const int32_t* blocks;
+  const int32_t* starts;       /* [B] or NULL */
+  const int32_t* lengths;      /* [B] or NULL */
+} mattn_selected;
+
+int mattn_selected_validate(const mattn_selected* p);
+
+/* Forward.  For a backward pass: o32 [B, Hkv, Lq, Hq / Hkv, D] and lse [B, Hkv, Lq,
+ * Hq / Hkv] float32 and lists (mattn_selected_lists_bytes, 256-byte aligned) are written
+ * and kept; otherwise all three NULL.  The workspace (256-byte aligned) may be used again
+ * when the call's work is done. */
+size_t mattn_selected_lists_bytes(const mattn_selected* p);
+size_t mattn_selected_fwd_workspace_bytes(const mattn_selected* p);
+int mattn_selected_fwd(const mattn_selected* p, const void* q, const void* k, const void* v, void* o, float* o32,
+                       float* lse, void* lists, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Backward of the same problem (the same blocks, starts and lengths): dq, dk and dv,
+ * every element written. */
+size_t mattn_selected_bwd_workspace_bytes(const mattn_selected* p);
+int mattn_selected_bwd(const mattn_selected* p, const void* q, const void* k, const void* v, const float* o32,
+                       const void* do_, const float* lse, const void* lists, void* workspace,
+                       size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
+
 /* Static text of a status code. */
 const char* mattn_strerror(int status);
 
 /* Library ABI version (bumped on any change of the structs, flags or functions above;
- * 10: rotary positions). */
+ * 10: rotary positions, block selection, attention over selected blocks). */
 int mattn_abi_version(void);
 
 #ifdef __cplusplus

@@ -44,7 +44,10 @@ EXPORTS = ("mattn_validate", "mattn_workspace_bytes", "mattn_bwd_workspace_bytes
            "mattn_fwd", "mattn_bwd",
            "mattn_bwd_stage", "mattn_strerror", "mattn_abi_version", "mattn_maskspec_validate",
            "mattn_tilemap_classify", "mattn_tilemap_bits", "mattn_bwd_noalloc", "mattn_copy_rows",
-           "mattn_rotary_fwd", "mattn_norm_rotary_bwd_workspace_bytes", "mattn_norm_rotary_bwd")
+           "mattn_rotary_fwd", "mattn_norm_rotary_bwd_workspace_bytes", "mattn_norm_rotary_bwd",
+           "mattn_block_means", "mattn_select_workspace_bytes", "mattn_select_blocks", "mattn_selected_validate",
+           "mattn_selected_lists_bytes", "mattn_selected_fwd_workspace_bytes", "mattn_selected_fwd",
+           "mattn_selected_bwd_workspace_bytes", "mattn_selected_bwd")
 SCRATCH_BYTES = 512 << 20  # MATTN_SCRATCH_BYTES
 BWD_PRE, BWD_DKDV, BWD_DQ = 0, 1, 2
 
@@ -111,6 +114,35 @@ class MattnRotary(ctypes.Structure):
     ]
 
 
+class MattnMeans(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("H", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("block_size", ctypes.c_int32), ("new_keys", ctypes.c_int32),
+        ("k_stride", _I64x3), ("k", ctypes.c_void_p), ("means", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+    ]
+
+
+class MattnSelect(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("nblk", ctypes.c_int32), ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("dtype", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("count", ctypes.c_int32), ("first", ctypes.c_int32), ("last", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("q_stride", _I64x3), ("m_stride", _I64x3), ("q", ctypes.c_void_p), ("means", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("blocks", ctypes.c_void_p),
+    ]
+
+
+class MattnSelected(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("Lq", ctypes.c_int32), ("Lk", ctypes.c_int32), ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("dtype", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("count", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("q_stride", _I64x3), ("k_stride", _I64x3), ("v_stride", _I64x3), ("o_stride", _I64x3),
+        ("do_stride", _I64x3), ("dq_stride", _I64x3), ("dk_stride", _I64x3), ("dv_stride", _I64x3),
+        ("blocks", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+    ]
+
+
 class MattnError(RuntimeError):
     def __init__(self, code: int, what: str = ""):
         self.code = code
@@ -174,6 +206,24 @@ def load():
         lib.mattn_norm_rotary_bwd_workspace_bytes.restype = ctypes.c_size_t
         lib.mattn_norm_rotary_bwd.argtypes = [R, vp, vp, vp, sz, vp]
         lib.mattn_norm_rotary_bwd.restype = ctypes.c_int
+        lib.mattn_block_means.argtypes = [ctypes.POINTER(MattnMeans), vp]
+        lib.mattn_block_means.restype = ctypes.c_int
+        C = ctypes.POINTER(MattnSelect)
+        lib.mattn_select_workspace_bytes.argtypes = [C]
+        lib.mattn_select_workspace_bytes.restype = sz
+        lib.mattn_select_blocks.argtypes = [C, vp, sz, vp]
+        lib.mattn_select_blocks.restype = ctypes.c_int
+        T = ctypes.POINTER(MattnSelected)
+        lib.mattn_selected_validate.argtypes = [T]
+        lib.mattn_selected_validate.restype = ctypes.c_int
+        for f in (lib.mattn_selected_lists_bytes, lib.mattn_selected_fwd_workspace_bytes,
+                  lib.mattn_selected_bwd_workspace_bytes):
+            f.argtypes = [T]
+            f.restype = sz
+        lib.mattn_selected_fwd.argtypes = [T, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.mattn_selected_fwd.restype = ctypes.c_int
+        lib.mattn_selected_bwd.argtypes = [T, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp, vp, vp, vp]
+        lib.mattn_selected_bwd.restype = ctypes.c_int
         lib.mattn_abi_version.argtypes = []
         lib.mattn_abi_version.restype = ctypes.c_int
         if lib.mattn_abi_version() != ABI_VERSION:

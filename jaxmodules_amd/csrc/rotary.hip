@@ -18,9 +18,7 @@
 // float32 product is off by 0.06 rad.  Sums, statistics and weight gradients are float32
 // (a thread's rows, then the groups of a workgroup, then the workgroups in a fixed
 // order: no atomics).
-#include <type_traits>
-
-#include "common.hpp"
+#include "elem.hpp"
 
 namespace mattn {
 namespace {
@@ -37,44 +35,6 @@ struct RotArgs {
   int pw_log2;   // positions of a workgroup
   int slots;     // lane slots of a row that hold columns
 };
-
-template <class Tag, int V>
-__device__ __forceinline__ void load_v(const void* base, int64_t e, float (&o)[V]) {
-  if constexpr (std::is_same_v<Tag, float>) {
-    const float* p = (const float*)base + e;
-    if constexpr (V == 4) {
-      const f32x4 x = *(const f32x4*)p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = x[i];
-    } else {
-      o[0] = *p;
-    }
-  } else {
-    const uint16_t* p = (const uint16_t*)base + e;
-    if constexpr (V == 8) {
-      const u32x4 x = *(const u32x4*)p;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = Elt<Tag>::to_f32(elt16(x, i));
-    } else {
-      o[0] = Elt<Tag>::to_f32(*p);
-    }
-  }
-}
-template <class Tag, int V>
-__device__ __forceinline__ void store_v(void* base, int64_t e, const float (&o)[V]) {
-  if constexpr (std::is_same_v<Tag, float>) {
-    float* p = (float*)base + e;
-    if constexpr (V == 4) *(f32x4*)p = f32x4{o[0], o[1], o[2], o[3]};
-    else *p = o[0];
-  } else {
-    uint16_t* p = (uint16_t*)base + e;
-    if constexpr (V == 8)
-      *(u32x4*)p = u32x4{Elt<Tag>::pack2(o[0], o[1]), Elt<Tag>::pack2(o[2], o[3]), Elt<Tag>::pack2(o[4], o[5]),
-                         Elt<Tag>::pack2(o[6], o[7])};
-    else
-      *p = (uint16_t)(Elt<Tag>::pack2(o[0], 0.f) & 0xffffu);
-  }
-}
 
 // The columns of lane slot s: a chunk of V at `a` and, where b >= 0, one at `b`;
 // rot: they hold V pairs, first pair V s.
@@ -399,7 +359,7 @@ int rot_launch(const mattn_rotary* p, float* part, hipStream_t st) {
   };
   using one = std::integral_constant<int, 1>;
   const auto pick = [&](auto tag) {
-    constexpr int V = std::is_same_v<decltype(tag), float> ? 4 : 8;
+    constexpr int V = kChunk<decltype(tag)>;
     if (vec) go(tag, std::integral_constant<int, V>{}, one{});
     else if (r.slots <= 64) go(tag, one{}, one{});
     else go(tag, one{}, std::integral_constant<int, 4>{});

@@ -1,0 +1,1285 @@
+// Attention of each query over the key blocks selected for it (mattn_selected_fwd,
+// mattn_selected_bwd).
+//
+//   O_q = sum_k P_qk V_k over the keys k of q's blocks that q sees,
+//   P_qk = exp(scale q.k - lse_q); the blocks are shared by the G query heads of a key head
+//   delta = dO . O, dS = P (dO . V - delta) scale; dQ = dS K, dK = dS^T Q, dV = P^T dO
+//
+// Two forms.  By blocks (prompts and training): the queries that selected a block are
+// listed once (list_* kernels), and a workgroup takes a block's keys and up to kRows rows
+// (query, head) of its list: whole matrix-core tiles whatever G is, K and V read once for
+// all of them.  A row's results of its blocks are joined by a second kernel: partial O
+// (and dQ) are float32 rows with a log-sum-exp, at [row][slot of the block in the query's
+// selection], so that nothing is added in an order of chance.  By queries (few rows, one
+// token of each sequence): a workgroup takes one query and key head, its waves the tiles
+// of 32 keys of its blocks.
+//
+// Infinite and NaN values: 0 times one is NaN in a matrix product, so a tile with such
+// values in rows that some of its queries (keys) must not see would spoil those.  The
+// products run with such values as 0 and mark the block, and the joining kernels add what
+// they give to the results that do see them, from the formula.
+//
+// Bound by the partial rows (by blocks): D * 4 bytes written and read for each (row,
+// block), 8 times the selected keys' own traffic at G = 4 and 64 keys a block; and by HBM
+// reads of K and V (by queries).
+#include <math.h>
+
+#include <initializer_list>
+
+#include "selected.hpp"
+
+namespace mattn {
+namespace {
+
+constexpr int kChunkQ = 256;    // queries a list workgroup takes
+constexpr int kRange = 1024;    // blocks a list workgroup takes
+constexpr int kRows = 512;      // rows (query, head) of a block that a forward or dQ workgroup takes
+constexpr int kRowsKV = 2048;   // rows that a dK/dV workgroup takes
+
+struct Desc {
+  int blk, row0;  // block (-1: idle) and first row of its list
+};
+
+struct SArgs {
+  mattn_selected p;
+  int G, nblk, bh_n;
+  float scale_log2;
+  const void *q, *k, *v, *dO;
+  void *o, *dq, *dk, *dv;
+  float *o32, *lse, *delta;  // [B * Hkv][Lq][G] rows (o32 [rows][D])
+  float *part, *plse;        // [rows][count][D], [rows][count]
+  float* kvpart;             // [B * Hkv][max_kv][2][KT][D]
+  int *odd, *kvodd;          // [B * Hkv][nblk]: infinite or NaN values were left out (of V or K; of Q or dO)
+  // lists
+  uint32_t* ok;              // [B * Hkv][Lq][words]: slots that count (visible, first of their block)
+  int* cnt;                  // [B * Hkv][nblk][chunks]: entries of a chunk, then their first index in the block's list
+  int* off;                  // [B * Hkv][nblk + 1]
+  int* kvoff;                // [B * Hkv][nblk + 1]: first dK/dV item of a block
+  int* ent;                  // [B * Hkv][Lq * count]: query * count + slot, by block, in the order of queries
+  Desc *tile, *kvtile;       // [B * Hkv][max_tiles], [B * Hkv][max_kv]
+  int words, chunks, max_tiles, max_kv, subs;  // subs: dK/dV key tiles of a block
+};
+
+__device__ __forceinline__ int keys_held(const mattn_selected& p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk;
+}
+__device__ __forceinline__ int64_t first_pos(const mattn_selected& p, int b) { return p.starts ? p.starts[b] : 0; }
+// Keys of sequence b that query q sees: those below the result.
+__device__ __forceinline__ int key_limit(const mattn_selected& p, int b, int q, int held, int64_t start) {
+  if (!p.causal) return held;
+  const int64_t e = start + q + 1;
+  return e < 0 ? 0 : e < held ? (int)e : held;
+}
+
+// ---- lists ----------------------------------------------------------------------------
+
+// The queries of a chunk that selected each block of a range, as bit masks in LDS; the
+// selection of query q: slots in order, entries outside [0, blocks seen) and repeated ones
+// left out.  FILL: the entries go to their places, otherwise the masks are counted.
+template <bool FILL>
+__global__ __attribute__((amdgpu_flat_work_group_size(kChunkQ, kChunkQ)))
+void list_entries(SArgs a) {
+  __shared__ uint32_t bits[kRange][kChunkQ / 32];
+  const mattn_selected& p = a.p;
+  const int bh = blockIdx.z, b = bh / p.Hkv, hk = bh % p.Hkv, chunk = blockIdx.x;
+  const int lo = blockIdx.y * kRange, n = min(kRange, a.nblk - lo);
+  const int t = threadIdx.x, q = chunk * kChunkQ + t;
+  for (int i = t; i < n * (kChunkQ / 32); i += kChunkQ) (&bits[0][0])[i] = 0u;
+  __syncthreads();
+  const int32_t* sel = p.blocks + (((int64_t)b * p.Lq + q) * p.Hkv + hk) * p.count;
+  const uint32_t mine = 1u << (t & 31);
+  int seen = 0;
+  if (q < p.Lq) {
+    const int lim = key_limit(p, b, q, keys_held(p, b), first_pos(p, b));
+    seen = (lim + p.block_size - 1) / p.block_size;
+    for (int w = 0; w < a.words; ++w) {
+      uint32_t good = 0u;
+      for (int c = 32 * w; c < min(32 * w + 32, p.count); ++c) {
+        const int j = sel[c] - lo;
+        if (j >= 0 && j < n && j + lo < seen && !(atomicOr(&bits[j][t >> 5], mine) & mine)) good |= 1u << (c & 31);
+      }
+      if constexpr (!FILL) {  // (ranges hold different blocks: their bits are joined in any order)
+        uint32_t* o = a.ok + ((int64_t)bh * p.Lq + q) * a.words + w;
+        if (gridDim.y == 1) *o = good;
+        else if (good) atomicOr(o, good);
+      }
+    }
+  }
+  __syncthreads();
+  if constexpr (!FILL) {
+    for (int j = t; j < n; j += kChunkQ) {
+      int s = 0;
+#pragma unroll
+      for (int w = 0; w < kChunkQ / 32; ++w) s += __popc(bits[j][w]);
+      a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] = s;
+    }
+  } else if (q < p.Lq) {
+    for (int w = 0; w < a.words; ++w) {
+      uint32_t good = a.ok[((int64_t)bh * p.Lq + q) * a.words + w];
+      for (; good; good &= good - 1) {
+        const int c = 32 * w + __ffs(good) - 1, j = sel[c] - lo;
+        if (j < 0 || j >= n) continue;
+        int r = __popc(bits[j][t >> 5] & (mine - 1));
+        for (int x = 0; x < (t >> 5); ++x) r += __popc(bits[j][x]);
+        a.ent[(int64_t)bh * p.Lq * p.count + a.off[(int64_t)bh * (a.nblk + 1) + lo + j] +
+              a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] + r] = q * p.count + c;
+      }
+    }
+  }
+}
+
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void list_clear(uint32_t* x, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) x[i] = 0u;
+}
+
+// inclusive sum over the lanes of a wave
+__device__ __forceinline__ int wave_scan(int x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Counts of a block's chunks to first indices; the block's total to off (a wave a block).
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void list_chunks(SArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (int64_t)a.bh_n * a.nblk) return;
+  int* c = a.cnt + i * a.chunks;
+  int sum = 0;
+  for (int x = 0; x < a.chunks; x += 64) {
+    const int v = x + lane < a.chunks ? c[x + lane] : 0, s = wave_scan(v, lane);
+    if (x + lane < a.chunks) c[x + lane] = sum + s - v;
+    sum += __shfl(s, 63);
+  }
+  if (lane == 0) a.off[i / a.nblk * (a.nblk + 1) + i % a.nblk] = sum;
+}
+
+// Totals to first entries, and the work items of the list kernels (a workgroup a head).
+constexpr int kScan = 1024;
+__global__ __attribute__((amdgpu_flat_work_group_size(kScan, kScan)))
+void list_items(SArgs a) {
+  __shared__ int wsum[3][kScan / 64];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  int* off = a.off + (int64_t)blockIdx.x * (a.nblk + 1);
+  int* kvoff = a.kvoff + (int64_t)blockIdx.x * (a.nblk + 1);
+  Desc* tile = a.tile + (int64_t)blockIdx.x * a.max_tiles;
+  Desc* kvtile = a.kvtile + (int64_t)blockIdx.x * a.max_kv;
+  int base[3] = {0, 0, 0};  // entries, tiles, dK/dV items before this range
+  for (int j0 = 0; j0 < a.nblk; j0 += kScan) {
+    const int j = j0 + t, n = j < a.nblk ? off[j] : 0;
+    const int rows = n * a.G;
+    const int v[3] = {n, (rows + kRows - 1) / kRows, (rows + kRowsKV - 1) / kRowsKV * a.subs};
+    int s[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      s[i] = wave_scan(v[i], lane);
+      if (lane == 63) wsum[i][w] = s[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      int before = base[i], all = 0;
+      for (int x = 0; x < kScan / 64; ++x) {
+        before += x < w ? wsum[i][x] : 0;
+        all += wsum[i][x];
+      }
+      s[i] += before - v[i];
+      base[i] += all;
+    }
+    __syncthreads();
+    if (j < a.nblk) {
+      off[j] = s[0];
+      kvoff[j] = s[2];
+      a.odd[(int64_t)blockIdx.x * a.nblk + j] = 0;
+    }
+    // the range's items, a wave a block at a time (values of the wave's own 64 blocks)
+    for (int x = 0; x < 64 && j0 + 64 * w + x < a.nblk; ++x) {
+      const int nt = __shfl(v[1], x), st = __shfl(s[1], x), nk = __shfl(v[2], x), sk = __shfl(s[2], x);
+      for (int i = lane; i < nt; i += 64) tile[st + i] = Desc{j0 + 64 * w + x, i * kRows};
+      // (key tile, rows): the tiles of a block next to each other
+      for (int i = lane; i < nk; i += 64) kvtile[sk + i] = Desc{j0 + 64 * w + x, i};
+    }
+  }
+  if (t == 0) {
+    off[a.nblk] = base[0];
+    kvoff[a.nblk] = base[2];
+  }
+  for (int i = base[1] + t; i < a.max_tiles; i += kScan) tile[i] = Desc{-1, 0};
+  for (int i = base[2] + t; i < a.max_kv; i += kScan) kvtile[i] = Desc{-1, 0};
+}
+
+// ---- by blocks ------------------------------------------------------------------------
+
+// Row r of a block's list: its query, slot and head.
+struct RowId {
+  int q, slot, g;
+};
+__device__ __forceinline__ RowId row_id(const SArgs& a, const int* list, int r) {
+  const int e = r / a.G, x = list[e], q = x / a.p.count;
+  return RowId{q, x - q * a.p.count, r - e * a.G};
+}
+
+// Rows k0 .. k0 + N - 1 of a [L, D] slice to LDS, zeros for rows at or past `end` and columns
+// at or past d.  Whether this thread's part holds an infinite or NaN value; CLEAN: 0 for those.
+template <class Tag, int D, int N, bool CLEAN>
+__device__ __forceinline__ bool stage_keys(char* lds, const void* base, int64_t stride, int64_t k0, int end, int d) {
+  bool odd = false;
+  using T = STile<Tag, D>;
+  constexpr int EC = 16 / SOp<Tag>::ES;  // elements of a chunk
+#pragma unroll
+  for (int i = 0; i < N * T::CPR / 256; ++i) {
+    const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (k0 + r < end && c * EC < d) v = *(const u32x4*)((const char*)base + SOp<Tag>::ES * ((k0 + r) * stride + c * EC));
+    if (SOp<Tag>::odd(v)) {
+      odd = true;
+      if constexpr (CLEAN) v = SOp<Tag>::finite16(v);
+    }
+    *(u32x4*)(lds + T::at(r, c)) = v;
+  }
+  return odd;
+}
+
+template <class Tag, int D>
+__device__ __forceinline__ void load_rows(typename SOp<Tag>::Frag (&f)[D / 16], const void* base, int64_t at, int hi, int d) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    const int c = 16 * s + 8 * hi;
+    f[s] = c < d ? SOp<Tag>::load((const char*)base + SOp<Tag>::ES * (at + c)) : SOp<Tag>::zero();
+  }
+}
+
+// O^T (register 4 j + i of tile mt: column 32 mt + 8 j + 4 hi + i of the lane's row) to a row of floats
+template <int D>
+__device__ __forceinline__ void put_row(float* out, const f32x16 (&acc)[D / 32], float s, int hi, int d) {
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 32 * mt + 8 * j + 4 * hi;
+      if (c < d)
+        *(f32x4*)(out + c) = f32x4{acc[mt][4 * j] * s, acc[mt][4 * j + 1] * s, acc[mt][4 * j + 2] * s, acc[mt][4 * j + 3] * s};
+    }
+}
+
+// Bits r of rows 8 (r / 4) + 4 hi + r % 4 (from row 0 of a 32-row tile) below `lim`.
+__device__ __forceinline__ uint32_t below(int lim, int hi) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = min(max(lim - 8 * j - 4 * hi, 0), 4);
+    m |= ((1u << n) - 1u) << (4 * j);
+  }
+  return m;
+}
+
+constexpr int kKT = 64;  // keys of a staged tile
+
+// Forward and dQ.  Four waves of 32 rows each (lane = row, both halves of a wave), 128 rows
+// at a time; the scores are formed transposed (rows of the MFMA result: keys), so that a
+// row's softmax is one lane's and its neighbour's, and P^T is the next product's operand
+// as it stands.  The first tile of a block of at most 64 keys stays in LDS for all rows.
+// P and dS are rounded to the inputs' type (as V and K are), sums are float32; the sum of
+// the weights adds them as rounded, so that O is a weighted mean of V's rows.
+template <class Tag, int D, bool GRAD>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void by_block_q(SArgs a) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  __shared__ __align__(16) char lds[2 * kKT * T::RB];
+  const mattn_selected& p = a.p;
+  const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const Desc desc = a.tile[(int64_t)bh * a.max_tiles + blockIdx.x / a.bh_n];
+  if (desc.blk < 0) return;
+  const int* off = a.off + (int64_t)bh * (a.nblk + 1) + desc.blk;
+  const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
+  const int rows = min((off[1] - off[0]) * a.G - desc.row0, kRows);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+  const int held = keys_held(p, b);
+  const int64_t start = first_pos(p, b), k0 = (int64_t)desc.blk * p.block_size;
+  const int inside = (int)min((int64_t)p.block_size, held - k0);  // keys of the block
+  const int tiles = (inside + kKT - 1) / kKT;
+  const char* kb = (const char*)a.k + O::ES * (b * p.k_stride[0] + hk * p.k_stride[2]);
+  const char* vb = (const char*)a.v + O::ES * (b * p.v_stride[0] + hk * p.v_stride[2]);
+  char *kt = lds, *vt = lds + kKT * T::RB;
+  bool odd = false;  // GRAD: the tile of K holds an infinite or NaN value
+
+  for (int r0 = 0; r0 < rows; r0 += 128) {
+    const int r = r0 + 32 * wave + l32;
+    const bool live = r < rows;
+    const RowId id = row_id(a, list, desc.row0 + min(r, rows - 1));
+    const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
+    const int h = hk * a.G + id.g;
+    typename O::Frag qf[D / 16], gf[GRAD ? D / 16 : 1];
+    load_rows<Tag, D>(qf, a.q, b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2], hi, p.D);
+    float lse = 0.f, delta = 0.f;
+    if constexpr (GRAD) {
+      load_rows<Tag, D>(gf, a.dO, b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2], hi, p.D);
+      lse = a.lse[row];
+      delta = a.delta[row];
+    }
+    const int64_t lim = key_limit(p, b, id.q, held, start) - k0;  // keys of the block the row sees
+    const int see = (int)min(lim, (int64_t)inside);
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
+    float m = NEG_INF, sum = 0.f, exact = 0.f;
+
+    for (int t = 0; t < tiles; ++t) {
+      if (tiles > 1 || r0 == 0) {
+        __syncthreads();
+        const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+        const bool vo = stage_keys<Tag, D, kKT, !GRAD>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+        if (GRAD ? ko : vo) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
+        if constexpr (GRAD) odd = __syncthreads_or(ko);
+        else __syncthreads();
+      }
+      const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
+      // (single floats from here on: of a 16-register result changed in a branch the compiler
+      // has written back registers of another value)
+      float s[2][16];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        f32x16 r16 = f32x16{};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(kt, 32 * x + l32, 2 * c + hi), qf[c], r16);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = r16[i];
+      }
+      uint32_t vis[2] = {0xffffu, 0xffffu};
+      if (part) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) vis[x] = below(see - t * kKT - 32 * x, hi);
+      }
+      if constexpr (!GRAD) {
+        float top = NEG_INF;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[x][i] = !part || ((vis[x] >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
+            top = fmaxf(top, s[x][i]);
+          }
+        top = fmaxf(m, wave_max32(top));
+        const float ref = top == NEG_INF ? 0.f : top;
+        const float keep = fast_exp2(m - ref);
+        m = top;
+        if (t > 0) {
+          sum *= keep;
+          exact *= keep;
+#pragma unroll
+          for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[mt][i] *= keep;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[x][i] = fast_exp2(s[x][i] - ref);
+            exact += s[x][i];
+          }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          f32x16 dp = f32x16{};
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) dp = O::mma32(T::row(vt, 32 * x + l32, 2 * c + hi), gf[c], dp);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float w = fast_exp2(s[x][i] * a.scale_log2 - lse) * (dp[i] - delta);
+            s[x][i] = !part || ((vis[x] >> i) & 1u) ? w : 0.f;
+          }
+        }
+      }
+      // P^T V^T, or dS^T K^T
+      const char* xt = GRAD ? kt : vt;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        typename O::Frag f[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = s[x][8 * j + i];
+          f[j] = O::pack(e);
+          if constexpr (!GRAD && O::ES == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
+          }
+        }
+        if (GRAD && odd) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(xt, 2 * x + j, mt, lane)), f[j], acc[mt]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(xt, 2 * x + j, mt, lane), f[j], acc[mt]);
+        }
+      }
+    }
+    const int64_t out = row * p.count + id.slot;
+    if constexpr (GRAD) {
+      if (live) put_row<D>(a.part + out * p.D, acc, p.scale, hi, p.D);
+    } else {
+      exact = wave_sum32(exact);
+      sum = O::ES == 2 ? wave_sum32(sum) : exact;
+      if (live) {
+        put_row<D>(a.part + out * p.D, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, hi, p.D);
+        if (hi == 0) a.plse[out] = exact > 0.f || exact != exact ? m + __log2f(exact) : NEG_INF;
+      }
+    }
+  }
+}
+
+// dK and dV of a key tile from up to kRowsKV rows: KT keys (64, or 128 for blocks of at
+// least 128), 64 rows at a time in LDS.  A wave holds 32 keys (lane = key) as operands in
+// registers and, with KT = 64, every other 32 rows; the scores' result has the rows along
+// its registers, so P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they
+// stand.  Float32 partial sums per item; the items of a block are added in order.
+template <class Tag, int D, int KT>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void by_block_kv(SArgs a) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  constexpr int NR = 64, KG = KT / 32, RG = 4 / KG;
+  __shared__ __align__(16) char lds[2 * NR * T::RB];
+  __shared__ __align__(16) float s_lse[NR], s_delta[NR];
+  __shared__ __align__(16) int s_see[NR];
+  const mattn_selected& p = a.p;
+  const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int64_t item = (int64_t)bh * a.max_kv + blockIdx.x / a.bh_n;
+  const Desc desc = a.kvtile[item];
+  if (desc.blk < 0) return;
+  const int* off = a.off + (int64_t)bh * (a.nblk + 1) + desc.blk;
+  const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
+  const int per = ((off[1] - off[0]) * a.G + kRowsKV - 1) / kRowsKV;  // items of a key tile
+  const int sub = desc.row0 / per, row0 = desc.row0 % per * kRowsKV;
+  const int rows = min((off[1] - off[0]) * a.G - row0, kRowsKV);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+  const int kg = wave % KG, rg = wave / KG;
+  const int held = keys_held(p, b);
+  const int64_t start = first_pos(p, b), k0 = (int64_t)desc.blk * p.block_size + sub * KT;
+  const int inside = (int)max(min((int64_t)min(p.block_size - sub * KT, KT), held - k0), (int64_t)0);  // keys of the tile
+  const int key = 32 * kg + l32;
+  char *qt = lds, *gt = lds + NR * T::RB;
+
+  typename O::Frag kf[D / 16], vf[D / 16];
+  if (key < inside) {
+    load_rows<Tag, D>(kf, a.k, b * p.k_stride[0] + hk * p.k_stride[2] + (k0 + key) * p.k_stride[1], hi, p.D);
+    load_rows<Tag, D>(vf, a.v, b * p.v_stride[0] + hk * p.v_stride[2] + (k0 + key) * p.v_stride[1], hi, p.D);
+  } else {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) kf[c] = vf[c] = O::zero();
+  }
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt) dk[mt] = dv[mt] = f32x16{};
+
+  for (int r0 = 0; r0 < rows; r0 += NR) {
+    __syncthreads();
+    constexpr int EC = 16 / O::ES, TPR = T::CPR < 16 ? T::CPR : 16;  // threads of a row
+#pragma unroll
+    for (int i = 0; i < NR * TPR / 256; ++i) {
+      const int x = i * 256 + threadIdx.x, r = x / TPR;
+      const bool live = r0 + r < rows;
+      const RowId id = row_id(a, list, row0 + min(r0 + r, rows - 1));
+      const int h = hk * a.G + id.g;
+      const char* qp = (const char*)a.q + O::ES * (b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2]);
+      const char* gp = (const char*)a.dO + O::ES * (b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2]);
+#pragma unroll
+      for (int ci = 0; ci < T::CPR / TPR; ++ci) {
+        const int c = x % TPR + ci * TPR;
+        u32x4 u = {0u, 0u, 0u, 0u}, w = {0u, 0u, 0u, 0u};
+        if (live && c * EC < p.D) {
+          u = *(const u32x4*)(qp + 16 * c);
+          w = *(const u32x4*)(gp + 16 * c);
+        }
+        *(u32x4*)(qt + T::at(r, c)) = u;
+        *(u32x4*)(gt + T::at(r, c)) = w;
+      }
+      if (x % TPR == 0) {
+        const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
+        s_lse[r] = live ? a.lse[row] : 0.f;
+        s_delta[r] = live ? a.delta[row] : 0.f;
+        s_see[r] = live ? (int)min(max((int64_t)key_limit(p, b, id.q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i32 = 0; i32 < NR / 32 / RG; ++i32) {
+      const int x = rg + i32 * RG;
+      if (r0 + 32 * x >= rows) continue;
+      uint32_t vis = 0u;
+      float s[16], dp[16];
+      {
+        f32x16 x16 = f32x16{}, y16 = f32x16{};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) x16 = O::mma32(T::row(qt, 32 * x + l32, 2 * c + hi), kf[c], x16);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) y16 = O::mma32(T::row(gt, 32 * x + l32, 2 * c + hi), vf[c], y16);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i] = x16[i];
+          dp[i] = y16[i];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 32 * x + 8 * j + 4 * hi;
+        const f32x4 l = *(const f32x4*)(s_lse + r), d = *(const f32x4*)(s_delta + r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool see = key < s_see[r + i];
+          vis |= (uint32_t)see << (4 * j + i);
+          const float w = fast_exp2(s[4 * j + i] * a.scale_log2 - l[i]);
+          s[4 * j + i] = see ? w : 0.f;
+          dp[4 * j + i] = see ? w * (dp[4 * j + i] - d[i]) : 0.f;
+        }
+      }
+      typename O::Frag pf[2], df[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float e[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = s[8 * j + i];
+          y[i] = dp[8 * j + i];
+        }
+        pf[j] = O::pack(e);
+        df[j] = O::pack(y);
+      }
+      const bool part = __any(vis != 0xffffu);
+      const auto add = [&](f32x16(&acc)[D / 32], const char* t, const typename O::Frag(&f)[2]) {
+        if (part && T::odd(t + 32 * x * T::RB, 32, lane)) {
+          a.kvodd[(int64_t)bh * a.nblk + desc.blk] = 1;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(t, 2 * x + j, mt, lane)), f[j], acc[mt]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(t, 2 * x + j, mt, lane), f[j], acc[mt]);
+        }
+      };
+      add(dv, gt, pf);
+      add(dk, qt, df);
+    }
+  }
+  // the row groups of a key, through LDS (a [32 keys][D] tile of floats for each key group), then to the item
+  float* out = a.kvpart + item * 2 * KT * p.D;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    f32x16(&acc)[D / 32] = w ? dv : dk;
+    const float sc = w ? 1.f : p.scale;
+    if constexpr (RG == 2) {
+      static_assert(2 * 32 * D * 4 <= sizeof(lds) || O::ES == 2);
+      // halves of the columns at a time where the tiles are of 16-bit values
+      constexpr int H = 2 * 32 * D * 4 <= 2 * NR * T::RB ? 1 : 2, MT = D / 32 / H;
+#pragma unroll
+      for (int part = 0; part < H; ++part) {
+        __syncthreads();
+        float* f = (float*)lds + kg * 32 * MT * 32;
+        if (rg == 1) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[(mt * 16 + i) * 64 + lane] = acc[part * MT + mt][i];
+        }
+        __syncthreads();
+        if (rg == 0) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[part * MT + mt][i] += f[(mt * 16 + i) * 64 + lane];
+        }
+      }
+      if (rg == 0) put_row<D>(out + ((int64_t)w * KT + key) * p.D, acc, sc, hi, p.D);
+    } else {
+      put_row<D>(out + ((int64_t)w * KT + key) * p.D, acc, sc, hi, p.D);
+    }
+  }
+}
+
+// ---- joining --------------------------------------------------------------------------
+
+// whether x holds in some lane of this lane's group of lpr
+__device__ __forceinline__ bool group_any(bool x, int lpr) {
+  const uint64_t m = __ballot(x);
+  const int lane = threadIdx.x & 63, first = lane & ~(lpr - 1);
+  return (m >> first) & (lpr == 64 ? ~0ull : (1ull << lpr) - 1);
+}
+
+// What the infinite and NaN values of a block's V (GRAD: K) give to a row's O (dQ), which
+// lpr lanes hold 4 columns each: weights from the formula, the row's lse known.
+template <class Tag, bool GRAD>
+__device__ __noinline__ void add_odd_keys(const SArgs& a, f32x4& o, float lse, int64_t row, int b, int hk, int h, int q, int blk,
+                                          int col, int lpr) {
+  const mattn_selected& p = a.p;
+  const int held = keys_held(p, b), lim = key_limit(p, b, q, held, first_pos(p, b));
+  const int64_t k0 = (int64_t)blk * p.block_size, k1 = min(k0 + p.block_size, (int64_t)lim);
+  const auto load = [&](const void* base, int64_t at, float(&x)[4]) {
+    if (col < p.D) load_v<Tag, 4>(base, at + col, x);
+    else x[0] = x[1] = x[2] = x[3] = 0.f;
+  };
+  const auto dot = [&](const float(&x)[4], const float(&y)[4]) {
+    float s = x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
+    for (int d = lpr >> 1; d; d >>= 1) s += __shfl_xor(s, d);
+    return s;
+  };
+  float qx[4];
+  load(a.q, b * p.q_stride[0] + q * p.q_stride[1] + h * p.q_stride[2], qx);
+  for (int64_t k = k0; k < k1; ++k) {
+    float kx[4], vx[4];
+    load(a.k, b * p.k_stride[0] + k * p.k_stride[1] + hk * p.k_stride[2], kx);
+    load(a.v, b * p.v_stride[0] + k * p.v_stride[1] + hk * p.v_stride[2], vx);
+    const float(&x)[4] = GRAD ? kx : vx;
+    bool odd[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd[i] = !__builtin_isfinite(x[i]);
+    if (!group_any(odd[0] || odd[1] || odd[2] || odd[3], lpr)) continue;
+    float w = fast_exp2(dot(qx, kx) * a.scale_log2 - lse);
+    if constexpr (GRAD) {
+      float gx[4];
+      load(a.dO, b * p.do_stride[0] + q * p.do_stride[1] + h * p.do_stride[2], gx);
+      w *= (dot(gx, vx) - a.delta[row]) * p.scale;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += odd[i] ? w * x[i] : 0.f;
+  }
+}
+
+// The same of the rows of a block's list for 4 columns of a key's dK (W = 0) or dV (W = 1).
+template <class Tag, int W>
+__device__ __noinline__ void add_odd_rows(const SArgs& a, float (&o)[4], int bh, int key, int blk, int col) {
+  const mattn_selected& p = a.p;
+  const int b = bh / p.Hkv, hk = bh % p.Hkv, held = keys_held(p, b);
+  const int* off = a.off + (int64_t)bh * (a.nblk + 1) + blk;
+  const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
+  const int64_t ka = b * p.k_stride[0] + key * p.k_stride[1] + hk * p.k_stride[2];
+  const int64_t va = b * p.v_stride[0] + key * p.v_stride[1] + hk * p.v_stride[2];
+  for (int r = 0; r < (off[1] - off[0]) * a.G; ++r) {
+    const RowId id = row_id(a, list, r);
+    if (key >= key_limit(p, b, id.q, held, first_pos(p, b))) continue;
+    const int h = hk * a.G + id.g;
+    const int64_t qa = b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2];
+    const int64_t ga = b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2];
+    float x[4];
+    load_v<Tag, 4>(W ? a.dO : a.q, (W ? ga : qa) + col, x);
+    if (__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3])) continue;
+    const auto dot = [&](const void* u, int64_t ua, const void* w, int64_t wa) {
+      float s = 0.f;
+      for (int c = 0; c < p.D; c += 4) {
+        float y[4], z[4];
+        load_v<Tag, 4>(u, ua + c, y);
+        load_v<Tag, 4>(w, wa + c, z);
+        s += y[0] * z[0] + y[1] * z[1] + y[2] * z[2] + y[3] * z[3];
+      }
+      return s;
+    };
+    const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
+    float w = fast_exp2(dot(a.q, qa, a.k, ka) * a.scale_log2 - a.lse[row]);
+    if constexpr (W == 0) w *= (dot(a.dO, ga, a.v, va) - a.delta[row]) * p.scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __builtin_isfinite(x[i]) ? 0.f : w * x[i];
+  }
+}
+
+// A row's partial results, 4 columns a lane: weighted by their log-sum-exp (forward), or
+// added (dQ).  Slots outside the selection's valid ones hold nothing and are not read.
+template <class Tag, bool GRAD>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void join_rows(SArgs a, int lpr_log2, int slots, bool all) {
+  const mattn_selected& p = a.p;
+  const int lpr = 1 << lpr_log2, lane = threadIdx.x & (lpr - 1), col = 4 * lane;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lpr_log2;
+  if (row >= (int64_t)a.bh_n * p.Lq * a.G) return;
+  const int g = (int)(row % a.G), q = (int)(row / a.G % p.Lq), bh = (int)(row / a.G / p.Lq);
+  const uint32_t* ok = a.ok + ((int64_t)bh * p.Lq + q) * a.words;
+  const float* part = a.part + row * slots * p.D;
+  const float* plse = a.plse + row * slots;
+  const auto valid = [&](int s) { return all || ((ok[s >> 5] >> (s & 31)) & 1u); };
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float lse = GRAD ? a.lse[row] : NEG_INF;
+  if constexpr (!GRAD) {
+    float m = NEG_INF;
+    bool nan = false;
+    for (int s = 0; s < slots; ++s)
+      if (valid(s)) {
+        m = fmaxf(m, plse[s]);
+        nan = nan || plse[s] != plse[s];
+      }
+    if (nan) m = __builtin_nanf("");
+    float sum = 0.f;
+    if (m != NEG_INF) {
+#pragma unroll 4
+      for (int s = 0; s < slots; ++s) {
+        if (!valid(s)) continue;
+        const float w = fast_exp2(plse[s] - m);
+        if (w == 0.f) continue;
+        sum += w;
+        if (col < p.D) {
+          const f32x4 x = *(const f32x4*)(part + (int64_t)s * p.D + col);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] += w * x[i];
+        }
+      }
+      const float r = 1.f / sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= r;
+      lse = m + __log2f(sum);
+    }
+  } else if (col < p.D) {
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) {
+      if (!valid(s)) continue;
+      const f32x4 x = *(const f32x4*)(part + (int64_t)s * p.D + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += x[i];
+    }
+  }
+  const int b = bh / p.Hkv, h = bh % p.Hkv * a.G + g;
+  if (!all) {
+    const int32_t* sel = p.blocks + (((int64_t)b * p.Lq + q) * p.Hkv + bh % p.Hkv) * p.count;
+    bool any = false;
+    for (int s = lane; s < slots; s += lpr) any = any || (valid(s) && a.odd[(int64_t)bh * a.nblk + sel[s]]);
+    if (group_any(any, lpr))
+      for (int s = 0; s < slots; ++s)
+        if (valid(s) && a.odd[(int64_t)bh * a.nblk + sel[s]]) add_odd_keys<Tag, GRAD>(a, o, lse, row, b, bh % p.Hkv, h, q, sel[s], col, lpr);
+  }
+  if (col < p.D) {
+    const int64_t* st = GRAD ? p.dq_stride : p.o_stride;
+    const float x[4] = {o[0], o[1], o[2], o[3]};
+    store_v<Tag, 4>(GRAD ? a.dq : a.o, b * st[0] + q * st[1] + h * st[2] + col, x);
+    if (!GRAD && a.o32) *(f32x4*)(a.o32 + row * p.D + col) = o;
+  }
+  if (!GRAD && lane == 0 && a.lse) a.lse[row] = lse;
+}
+
+// delta = dO . O of each row, 4 columns a lane; no block marked yet
+template <class Tag>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void row_delta(SArgs a, int lpr_log2) {
+  const mattn_selected& p = a.p;
+  const int lpr = 1 << lpr_log2, lane = threadIdx.x & (lpr - 1), col = 4 * lane;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)a.bh_n * a.nblk; i += (int64_t)gridDim.x * 256)
+    a.odd[i] = a.kvodd[i] = 0;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lpr_log2;
+  if (row >= (int64_t)a.bh_n * p.Lq * a.G) return;
+  const int g = (int)(row % a.G), q = (int)(row / a.G % p.Lq), bh = (int)(row / a.G / p.Lq);
+  const int b = bh / p.Hkv, h = bh % p.Hkv * a.G + g;
+  float s = 0.f;
+  if (col < p.D) {
+    float x[4];
+    load_v<Tag, 4>(a.dO, b * p.do_stride[0] + q * p.do_stride[1] + h * p.do_stride[2] + col, x);
+    const f32x4 o = *(const f32x4*)(a.o32 + row * p.D + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += x[i] * o[i];
+  }
+  for (int o = lpr >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) a.delta[row] = s;
+}
+
+// dK and dV of each key: the items of its block in order, 4 columns a thread; zeros for keys no query saw.
+template <class Tag>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void join_keys(SArgs a, int KT) {
+  const mattn_selected& p = a.p;
+  const int cpr = p.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int col = 4 * (int)(i % cpr);
+  const int64_t kk = i / cpr;
+  if (kk >= p.Lk) return;
+  const int key = (int)kk, w = blockIdx.y & 1, bh = blockIdx.y >> 1, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int blk = key / p.block_size, in = key % p.block_size, sub = in / KT;
+  const int* kvoff = a.kvoff + (int64_t)bh * (a.nblk + 1) + blk;
+  const int per = (kvoff[1] - kvoff[0]) / a.subs;
+  const float* part = a.kvpart + (((int64_t)bh * a.max_kv + kvoff[0] + sub * per) * 2 + w) * KT * p.D + (int64_t)(in % KT) * p.D + col;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int x = 0; x < per; ++x) {
+    const f32x4 v = *(const f32x4*)(part + (int64_t)x * 2 * KT * p.D);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += v[e];
+  }
+  if (a.kvodd[(int64_t)bh * a.nblk + blk]) {
+    if (w) add_odd_rows<Tag, 1>(a, o, bh, key, blk, col);
+    else add_odd_rows<Tag, 0>(a, o, bh, key, blk, col);
+  }
+  const int64_t* st = w ? p.dv_stride : p.dk_stride;
+  store_v<Tag, 4>(w ? a.dv : a.dk, b * st[0] + kk * st[1] + hk * st[2] + col, o);
+}
+
+// ---- by queries -----------------------------------------------------------------------
+
+// One query, key head, 16 of its query heads and a part of its keys: the workgroup's four
+// waves take tiles of 32 keys in turn.  Keys go straight from memory to operands (16 rows
+// of 64 bytes a load), values through LDS for the transposed reads.  All rows of a tile
+// see the same keys, so values past them are set to zero.  Bound by HBM.
+// LDS written by the wave's lanes is read by its other lanes after this
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kMaxSel = 1024;  // blocks of a query
+template <class Tag, int D>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+void by_query(SArgs a, int splits, int hgroups) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  constexpr int VB = 32 * T::RB, JB = 16 * D * 4;  // a wave's values; its heads' sums
+  __shared__ __align__(16) char lds[4 * (VB > JB ? VB : JB)];
+  __shared__ int list[kMaxSel];
+  __shared__ int n_list;
+  __shared__ float s_m[4][16], s_l[4][16], s_e[4][16];
+  const mattn_selected& p = a.p;
+  int x = blockIdx.x;
+  const int split = x % splits;
+  x /= splits;
+  const int hg = x % hgroups;
+  x /= hgroups;
+  const int bh = x % a.bh_n, q = x / a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int held = keys_held(p, b);
+  const int lim = key_limit(p, b, q, held, first_pos(p, b));
+  const int seen = (lim + p.block_size - 1) / p.block_size;
+  const int32_t* sel = p.blocks + (((int64_t)b * p.Lq + q) * p.Hkv + hk) * p.count;
+  if (wave == 0) {  // the valid blocks, in their order; repeated ones left out
+    int n = 0;
+    bool rising = true;
+    for (int c = 0; c < p.count; c += 64) {
+      const int j = c + lane < p.count ? sel[c + lane] : -1;
+      const bool good = j >= 0 && j < seen;
+      const uint64_t m = __ballot(good);
+      const int at = n + __builtin_popcountll(m & ((1ull << lane) - 1));
+      if (good) list[at] = j;
+      n += __builtin_popcountll(m);
+    }
+    wave_sync();
+    for (int c = 0; c < n; c += 64) {
+      const int j = c + lane < n ? list[c + lane] : 0x7fffffff;
+      const int before = c + lane == 0 ? -1 : c + lane < n ? list[c + lane - 1] : -1;
+      if (!__all(j > before)) rising = false;
+    }
+    if (!rising) {  // compact what occurs for the first time
+      int kept = 0;
+      for (int c = 0; c < n; ++c) {
+        const int j = list[c];
+        bool dup = false;
+        for (int i = lane; i < kept; i += 64) dup = dup || list[i] == j;
+        if (!__any(dup)) {
+          if (lane == 0) list[kept] = j;
+          ++kept;
+        }
+        wave_sync();
+      }
+      n = kept;
+    }
+    if (lane == 0) n_list = n;
+  }
+  const int h0 = 16 * hg, nh = min(16, a.G - h0);
+  typename O::Frag qf[D / 32];
+  {
+    const int64_t at = b * p.q_stride[0] + q * p.q_stride[1] + (int64_t)(hk * a.G + h0 + min(l16, nh - 1)) * p.q_stride[2];
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      const int c = 32 * s + 8 * g;
+      qf[s] = c < p.D ? O::load((const char*)a.q + O::ES * (at + c)) : O::zero();
+    }
+  }
+  __syncthreads();
+  const int bs = p.block_size, nk = n_list * bs;  // keys in the list's order
+  const int tiles = (nk + 31) / 32, per = (tiles + splits - 1) / splits;
+  const int t1 = min((split + 1) * per, tiles);
+  const char* kb = (const char*)a.k + O::ES * (b * p.k_stride[0] + hk * p.k_stride[2]);
+  const char* vb = (const char*)a.v + O::ES * (b * p.v_stride[0] + hk * p.v_stride[2]);
+  char* vt = lds + wave * VB;
+  f32x4 acc[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = NEG_INF, sum = 0.f, exact = 0.f;
+  for (int t = split * per + wave; t < t1; t += 4) {
+    // key of each of the tile's 32 places (lane % 32), -1 where there is none
+    const int at = 32 * t + (lane & 31);
+    const int j = at < nk ? list[at / bs] : 0;
+    const int kl = at < nk && j * (int64_t)bs + at % bs < lim ? j * bs + at % bs : -1;
+    typename O::Frag kf[2][D / 32];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = __shfl(kl, 16 * u + l16);
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        const int c = 32 * s + 8 * g;
+        kf[u][s] = key >= 0 && c < p.D ? O::load(kb + O::ES * (key * p.k_stride[1] + c)) : O::zero();
+      }
+    }
+    constexpr int EC = 16 / O::ES;
+    u32x4 vx[VB / 1024];
+#pragma unroll
+    for (int i = 0; i < VB / 1024; ++i) {
+      const int y = 64 * i + lane, key = __shfl(kl, y / T::CPR), c = y % T::CPR;
+      vx[i] = key >= 0 && c * EC < p.D ? *(const u32x4*)(vb + O::ES * (key * p.v_stride[1]) + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+    }
+    f32x4 s2[2];
+    float top = NEG_INF;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s2[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) s2[u] = O::mma16(kf[u][s], qf[s], s2[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = __shfl(kl, 16 * u + 4 * g + i);
+        s2[u][i] = key >= 0 ? s2[u][i] * a.scale_log2 : NEG_INF;
+        top = fmaxf(top, s2[u][i]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    const float ref = top == NEG_INF ? 0.f : top, keep = fast_exp2(m - ref);
+    m = top;
+    sum *= keep;
+    exact *= keep;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[d][i] *= keep;
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      e[i] = fast_exp2(s2[i >> 2][i & 3] - ref);
+      exact += e[i];
+    }
+    const typename O::Frag pf = O::pack(e);
+    if constexpr (O::ES == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, pf), i));
+    }
+#pragma unroll
+    for (int i = 0; i < VB / 1024; ++i) {
+      const int y = 64 * i + lane;
+      *(u32x4*)(vt + T::at(y / T::CPR, y % T::CPR)) = vx[i];
+    }
+    wave_sync();
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[d] = O::mma16(T::tr16(vt, d, lane), pf, acc[d]);
+    wave_sync();
+  }
+  exact += __shfl_xor(exact, 16);
+  exact += __shfl_xor(exact, 32);
+  if constexpr (O::ES == 2) {
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+  } else {
+    sum = exact;
+  }
+  // the waves' results: [column][head] sums of each in LDS
+  __syncthreads();
+  float* f = (float*)lds + wave * 16 * D;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) *(f32x4*)(f + l16 * D + 16 * d + 4 * g) = acc[d];
+  if (g == 0) {
+    s_m[wave][l16] = m;
+    s_l[wave][l16] = sum;
+    s_e[wave][l16] = exact;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * (D / 4); i += 256) {
+    const int h = i / (D / 4), c = 4 * (i % (D / 4));
+    float top = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+    const float ref = top == NEG_INF ? 0.f : top;
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, ex = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float y = fast_exp2(s_m[w][h] - ref);
+      l += y * s_l[w][h];
+      ex += y * s_e[w][h];
+      const f32x4 v = *(const f32x4*)((float*)lds + (w * 16 + h) * D + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += y * v[e];
+    }
+    const float r = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= r;
+    if (c >= p.D) continue;
+    const int64_t row = ((int64_t)bh * p.Lq + q) * a.G + h0 + h;
+    const float lse = ex > 0.f || ex != ex ? ref + __log2f(ex) : NEG_INF;
+    if (splits > 1) {
+      *(f32x4*)(a.part + (row * splits + split) * p.D + c) = f32x4{o[0], o[1], o[2], o[3]};
+      if (c == 0) a.plse[row * splits + split] = lse;
+    } else {
+      store_v<Tag, 4>(a.o, b * p.o_stride[0] + q * p.o_stride[1] + (int64_t)(hk * a.G + h0 + h) * p.o_stride[2] + c, o);
+      if (a.o32) *(f32x4*)(a.o32 + row * p.D + c) = f32x4{o[0], o[1], o[2], o[3]};
+      if (c == 0 && a.lse) a.lse[row] = lse;
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+int key_tile(const mattn_selected* p) { return p->block_size >= 128 ? 128 : 64; }
+
+int sel_check(const mattn_selected* p) {
+  if (!p) return MATTN_ERR_NULL;
+  if (p->B <= 0 || p->Lq <= 0 || p->Lk <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv) return MATTN_ERR_SHAPE;
+  if (p->D <= 0 || p->D > 128 || p->D % 8) return MATTN_ERR_HEAD_DIM;
+  if (p->block_size <= 0 || p->block_size % 16 || p->count <= 0 || p->count > kMaxSel) return MATTN_ERR_SHAPE;
+  if (p->dtype != MATTN_BF16 && p->dtype != MATTN_F16 && p->dtype != MATTN_F32) return MATTN_ERR_DTYPE;
+  if (!isfinite(p->scale)) return MATTN_ERR_SHAPE;
+  if (!p->blocks) return MATTN_ERR_NULL;
+  const int es = p->dtype == MATTN_F32 ? 4 : 2;
+  for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride, p->o_stride, p->do_stride, p->dq_stride, p->dk_stride, p->dv_stride})
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || (s[i] * es) % 16) return MATTN_ERR_STRIDE;
+  const int64_t lim = 1ll << 31, bh = (int64_t)p->B * p->Hkv, G = p->Hq / p->Hkv;
+  if (p->Lk + (int64_t)p->block_size >= lim || (int64_t)p->Lq * p->count * G >= lim || bh > 32767 || bh * p->Lq * G >= lim / 64)
+    return MATTN_ERR_TOO_LARGE;
+  return MATTN_OK;
+}
+
+struct SPlan {
+  bool by_query;
+  int splits, hgroups;
+};
+
+// Which form serves the forward, and its splits.
+SPlan sel_plan(const mattn_selected* p) {
+  const int64_t G = p->Hq / p->Hkv, bh = (int64_t)p->B * p->Hkv;
+  SPlan s;
+  s.hgroups = (int)cdiv(G, 16);
+  const int64_t wgs = bh * p->Lq * s.hgroups, tiles = cdiv((int64_t)p->count * p->block_size, 32);
+  s.by_query = p->Lq <= 16;
+  s.splits = 1;
+  while (s.splits < 32 && wgs * s.splits < 512 && tiles / (2 * s.splits) >= 4) s.splits *= 2;
+  return s;
+}
+
+struct SLayout {
+  // lists: kept for the backward
+  size_t ok, off, kvoff, ent, tile, kvtile, lists;
+  // workspace
+  size_t cnt, odd, part, plse, fwd;                   // forward
+  size_t delta, dqpart, kvpart, bodd, kvodd, bwd;  // backward
+  int words, chunks, nblk, max_tiles, max_kv, subs;
+};
+
+SLayout sel_layout(const mattn_selected* p) {
+  SLayout l{};
+  const int64_t bh = (int64_t)p->B * p->Hkv, G = p->Hq / p->Hkv, rows = bh * p->Lq * G;
+  l.nblk = (int)cdiv(p->Lk, p->block_size);
+  l.words = (p->count + 31) / 32;
+  l.chunks = (int)cdiv(p->Lq, kChunkQ);
+  l.subs = (int)cdiv(p->block_size, key_tile(p));
+  const int64_t most = (int64_t)p->Lq * p->count;  // entries of a head
+  const int64_t used = l.nblk < most ? l.nblk : most;
+  l.max_tiles = (int)(most * G / kRows + used);
+  l.max_kv = (int)((most * G / kRowsKV + used) * l.subs);
+  size_t x = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t at = x;
+    x += align256(bytes);
+    return at;
+  };
+  l.ok = take(bh * p->Lq * l.words * 4);
+  l.off = take(bh * (l.nblk + 1) * 4);
+  l.kvoff = take(bh * (l.nblk + 1) * 4);
+  l.ent = take(bh * most * 4);
+  l.tile = take(bh * l.max_tiles * sizeof(Desc));
+  l.kvtile = take(bh * l.max_kv * sizeof(Desc));
+  l.lists = x;
+  x = 0;
+  const SPlan s = sel_plan(p);
+  const int64_t slots = s.by_query ? (s.splits > 1 ? s.splits : 0) : p->count;
+  l.cnt = take(bh * l.nblk * l.chunks * 4);
+  l.odd = take(bh * l.nblk * 4);
+  l.part = take(rows * slots * p->D * 4);
+  l.plse = take(rows * slots * 4);
+  l.fwd = x;
+  x = 0;
+  l.delta = take(rows * 4);
+  l.dqpart = take(rows * p->count * p->D * 4);
+  l.kvpart = take(bh * l.max_kv * 2 * key_tile(p) * p->D * 4);
+  l.bodd = take(bh * l.nblk * 4);
+  l.kvodd = take(bh * l.nblk * 4);
+  l.bwd = x;
+  return l;
+}
+
+SArgs sel_args(const mattn_selected* p, const SLayout& l, void* lists) {
+  SArgs a{};
+  a.p = *p;
+  a.G = p->Hq / p->Hkv;
+  a.nblk = l.nblk;
+  a.bh_n = p->B * p->Hkv;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.words = l.words;
+  a.chunks = l.chunks;
+  a.max_tiles = l.max_tiles;
+  a.max_kv = l.max_kv;
+  a.subs = l.subs;
+  char* c = (char*)lists;
+  if (c) {
+    a.ok = (uint32_t*)(c + l.ok);
+    a.off = (int*)(c + l.off);
+    a.kvoff = (int*)(c + l.kvoff);
+    a.ent = (int*)(c + l.ent);
+    a.tile = (Desc*)(c + l.tile);
+    a.kvtile = (Desc*)(c + l.kvtile);
+  }
+  return a;
+}
+
+void make_lists(const SArgs& a, hipStream_t st) {
+  const dim3 grid(a.chunks, (uint32_t)cdiv(a.nblk, kRange), a.bh_n);
+  if (grid.y > 1) {
+    const int64_t n = (int64_t)a.bh_n * a.p.Lq * a.words;
+    hipLaunchKernelGGL(list_clear, dim3((uint32_t)(cdiv(n, 256) < 1024 ? cdiv(n, 256) : 1024)), dim3(256), 0, st, a.ok, n);
+  }
+  hipLaunchKernelGGL((list_entries<false>), grid, dim3(kChunkQ), 0, st, a);
+  hipLaunchKernelGGL(list_chunks, dim3((uint32_t)cdiv((int64_t)a.bh_n * a.nblk, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(list_items, dim3(a.bh_n), dim3(kScan), 0, st, a);
+  hipLaunchKernelGGL((list_entries<true>), grid, dim3(kChunkQ), 0, st, a);
+}
+
+int lanes_log2(int D) {  // lanes of 4 columns that hold a row
+  int l = 1;
+  while ((4 << l) < D) ++l;
+  return l;
+}
+
+template <class F>
+void with_type(int dtype, F&& f) {
+  if (dtype == MATTN_BF16) f(bf16_tag{});
+  else if (dtype == MATTN_F16) f(f16_tag{});
+  else f(float{});
+}
+template <class F>
+void with_dim(int D, F&& f) {
+  if (D <= 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+bool misaligned(std::initializer_list<const void*> ps, unsigned mask) {
+  for (const void* x : ps)
+    if ((uintptr_t)x & mask) return true;
+  return false;
+}
+
+}  // namespace
+}  // namespace mattn
+
+using namespace mattn;
+
+extern "C" int mattn_selected_validate(const mattn_selected* p) { return sel_check(p); }
+
+extern "C" size_t mattn_selected_lists_bytes(const mattn_selected* p) { return sel_check(p) ? 0 : sel_layout(p).lists; }
+
+extern "C" size_t mattn_selected_fwd_workspace_bytes(const mattn_selected* p) {
+  if (sel_check(p)) return 0;
+  const SLayout l = sel_layout(p);
+  return sel_plan(p).by_query ? l.fwd : l.fwd + l.lists;
+}
+
+extern "C" size_t mattn_selected_bwd_workspace_bytes(const mattn_selected* p) { return sel_check(p) ? 0 : sel_layout(p).bwd; }
+
+extern "C" int mattn_selected_fwd(const mattn_selected* p, const void* q, const void* k, const void* v, void* o, float* o32,
+                                  float* lse, void* lists, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = sel_check(p)) return rc;
+  if (!q || !k || !v || !o) return MATTN_ERR_NULL;
+  const bool grads = lists != nullptr;
+  if (grads && (!o32 || !lse)) return MATTN_ERR_NULL;
+  const size_t need = mattn_selected_fwd_workspace_bytes(p);
+  if (need > 0 && !workspace) return MATTN_ERR_NULL;
+  if (workspace_bytes < need) return MATTN_ERR_WORKSPACE;
+  if (misaligned({q, k, v, o, o32}, 15) || misaligned({lists, workspace}, 255)) return MATTN_ERR_STRIDE;
+  const SLayout l = sel_layout(p);
+  const SPlan s = sel_plan(p);
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  SArgs a = sel_args(p, l, lists ? lists : ws ? ws + l.fwd : nullptr);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.o32 = grads ? o32 : nullptr;
+  a.lse = grads ? lse : nullptr;
+  a.cnt = (int*)(ws + l.cnt);
+  a.odd = (int*)(ws + l.odd);
+  a.part = (float*)(ws + l.part);
+  a.plse = (float*)(ws + l.plse);
+  if (grads || !s.by_query) make_lists(a, st);
+  const int ll = lanes_log2(p->D);
+  const int64_t rows = (int64_t)a.bh_n * p->Lq * a.G;
+  const dim3 join((uint32_t)cdiv(rows << ll, 256));
+  with_type(p->dtype, [&](auto tag) {
+    using Tag = decltype(tag);
+    with_dim(p->D, [&](auto dim) {
+      constexpr int D = decltype(dim)::value;
+      if (s.by_query)
+        hipLaunchKernelGGL((by_query<Tag, D>), dim3((uint32_t)(a.bh_n * p->Lq * s.hgroups * s.splits)), dim3(256), 0, st, a, s.splits, s.hgroups);
+      else
+        hipLaunchKernelGGL((by_block_q<Tag, D, false>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
+    });
+    if (!s.by_query) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, p->count, false);
+    else if (s.splits > 1) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, s.splits, true);
+  });
+  return hipGetLastError() == hipSuccess ? MATTN_OK : MATTN_ERR_LAUNCH;
+}
+
+extern "C" int mattn_selected_bwd(const mattn_selected* p, const void* q, const void* k, const void* v, const float* o32,
+                                  const void* do_, const float* lse, const void* lists, void* workspace,
+                                  size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream) {
+  if (const int rc = sel_check(p)) return rc;
+  if (!q || !k || !v || !o32 || !do_ || !lse || !lists || !workspace || !dq || !dk || !dv) return MATTN_ERR_NULL;
+  const SLayout l = sel_layout(p);
+  if (workspace_bytes < l.bwd) return MATTN_ERR_WORKSPACE;
+  if (misaligned({q, k, v, o32, do_, dq, dk, dv}, 15) || misaligned({lists, workspace}, 255)) return MATTN_ERR_STRIDE;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  SArgs a = sel_args(p, l, const_cast<void*>(lists));
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.dO = do_;
+  a.o32 = const_cast<float*>(o32);
+  a.lse = const_cast<float*>(lse);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.delta = (float*)(ws + l.delta);
+  a.part = (float*)(ws + l.dqpart);
+  a.kvpart = (float*)(ws + l.kvpart);
+  a.odd = (int*)(ws + l.bodd);
+  a.kvodd = (int*)(ws + l.kvodd);
+  const int ll = lanes_log2(p->D);
+  const int64_t rows = (int64_t)a.bh_n * p->Lq * a.G;
+  const dim3 join((uint32_t)cdiv(rows << ll, 256));
+  const int KT = key_tile(p);
+  const dim3 keys((uint32_t)cdiv((int64_t)p->Lk * (p->D / 4), 256), 2 * a.bh_n);
+  with_type(p->dtype, [&](auto tag) {
+    using Tag = decltype(tag);
+    hipLaunchKernelGGL((row_delta<Tag>), join, dim3(256), 0, st, a, ll);
+    with_dim(p->D, [&](auto dim) {
+      constexpr int D = decltype(dim)::value;
+      hipLaunchKernelGGL((by_block_q<Tag, D, true>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
+      if (KT == 128) hipLaunchKernelGGL((by_block_kv<Tag, D, 128>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((by_block_kv<Tag, D, 64>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(256), 0, st, a);
+    });
+    hipLaunchKernelGGL((join_rows<Tag, true>), join, dim3(256), 0, st, a, ll, p->count, false);
+    hipLaunchKernelGGL((join_keys<Tag>), keys, dim3(256), 0, st, a, KT);
+  });
+  return hipGetLastError() == hipSuccess ? MATTN_OK : MATTN_ERR_LAUNCH;
+}

@@ -1,0 +1,434 @@
+"""Block means, block selection and attention over selected blocks (GPU) against float64
+loops on the CPU (tests/selected_oracle.py, which derives the tolerances)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import selected_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+def _normal(gen, *shape, dtype="float32", f=1.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * f).to(getattr(torch, dtype))
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---- means -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("L,bs,H,d", [(1, 16, 1, 8), (130, 64, 3, 64), (257, 32, 2, 128), (100, 128, 5, 96), (63, 16, 2, 20),
+                                      (33, 16, 1, 5), (2049, 1024, 1, 64)])
+def test_block_means(dtype, L, bs, H, d):
+    import jaxmodules_amd as jm
+
+    k = _normal(_gen(L), 3, L, H, d, dtype=dtype)
+    lengths = _ints(L, max(L // 2, 1), 0)
+    for n in (None, lengths, _ints(L + 5, -3, 1)):
+        got = jm.block_means(k, bs, n)
+        want = so.means(k, bs, n)
+        assert got.dtype == torch.float32
+        # one rounding of a float64 sum (whose own error is far below a float32 step)
+        assert ((got.cpu().double() - want).abs() <= 2.0 ** -24 * (1 + 1e-6) * want.abs() + 1e-12 * k.double().abs().max().item()).all()
+
+
+def test_block_means_of_views():
+    import jaxmodules_amd as jm
+
+    x = _normal(_gen(1), 2, 3, 100, 64)
+    flat = _normal(_gen(2), 2 * 100 * 3 * 64 + 1)
+    for k in (x.transpose(1, 2), flat[1:].view(2, 100, 3, 64), x.transpose(1, 2)[..., ::2]):
+        assert torch.equal(jm.block_means(k, 16), jm.block_means(k.contiguous(), 16))
+
+
+@pytest.mark.parametrize("new", [1, 4, 16, 40])
+def test_block_means_update_writes_the_touched_blocks_alone(new):
+    import jaxmodules_amd as jm
+
+    k = _normal(_gen(3), 5, 100, 2, 64, dtype="bfloat16")
+    lengths = _ints(100, 48, 49, 3, 0)
+    full = jm.block_means(k, 16, lengths)
+    out = torch.full_like(full, 7.0)
+    assert jm.block_means(k, 16, lengths, out=out, new=new) is out
+    for b, n in enumerate((100, 48, 49, 3, 0)):
+        for j in range(full.shape[1]):
+            touched = j * 16 < n and (j + 1) * 16 > n - new
+            assert torch.equal(out[b, j], full[b, j] if touched else torch.full_like(full[b, j], 7.0)), (b, j)
+
+
+# ---- selection -------------------------------------------------------------------------
+
+
+SELECTIONS = [
+    # B, N, Hq, Hkv, d, L, bs, count, first, last
+    (1, 1, 1, 1, 8, 16, 16, 1, 0, 1), (2, 130, 4, 2, 64, 130, 16, 4, 1, 1), (1, 300, 8, 1, 128, 300, 16, 7, 0, 0),
+    (2, 70, 2, 2, 96, 70, 16, 16, 1, 2), (1, 500, 3, 3, 40, 500, 16, 5, 2, 3), (1, 2100, 2, 1, 64, 2100, 16, 9, 1, 1),
+    (1, 9, 4, 2, 20, 2500, 16, 33, 1, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("case", SELECTIONS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_select_blocks(case, causal, dtype):
+    import jaxmodules_amd as jm
+
+    B, N, Hq, Hkv, d, L, bs, count, first, last = case
+    gen = _gen(N + d)
+    q, k = _normal(gen, B, N, Hq, d, dtype=dtype), _normal(gen, B, L, Hkv, d, dtype=dtype)
+    m = jm.block_means(k, bs)
+    got = jm.select_blocks(q, m, bs, count, is_causal=causal, first=first, last=last)
+    assert torch.equal(got.cpu(), so.select(q, m, bs, count, causal, first, last)[0])
+
+
+@pytest.mark.parametrize("N", [1, 3, 8, 20])
+def test_select_for_served_tokens(N):
+    import jaxmodules_amd as jm
+
+    gen = _gen(N)
+    q, m = _normal(gen, 5, N, 4, 64, dtype="bfloat16"), _normal(gen, 5, 70, 2, 64)
+    lengths = _ints(70 * 16, 500, 17, 16, 0)
+    starts = lengths - N
+    for kw in (dict(starts=starts, lengths=lengths), dict(starts=starts), dict(lengths=lengths),
+               dict(lengths=lengths, is_causal=False), dict(starts=_ints(-5, 5000, 0, 1, 2))):
+        got = jm.select_blocks(q, m, 16, 6, **kw)
+        want = so.select(q, m, 16, 6, kw.get("is_causal", True), 1, 1, kw.get("starts"), kw.get("lengths"))[0]
+        assert torch.equal(got.cpu(), want), kw
+
+
+@pytest.mark.parametrize("nblk", [100, 500, 1900, 5000])
+@pytest.mark.parametrize("N", [2, 40])
+def test_select_many_blocks_ties_and_odd_values(nblk, N):
+    """Every form of the choice; equal means (ties to the lower index), zeros of both
+    signs, infinities and NaN."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(nblk)
+    m = torch.randint(-1, 2, (1, nblk, 1, 8), generator=gen, device="cuda").float()  # few distinct scores
+    q = torch.randint(-1, 2, (1, N, 2, 8), generator=gen, device="cuda").float()
+    m[0, 7] = -0.0
+    for count in (3, 64, nblk // 2 if nblk < 2000 else 999):
+        got = jm.select_blocks(q, m, 16, count, is_causal=False)
+        assert torch.equal(got.cpu(), so.select(q, m, 16, count, False)[0])
+    m[0, 11, 0, 0] = float("nan")
+    m[0, 12, 0, 1], m[0, 13, 0, 2] = float("inf"), -float("inf")
+    got = jm.select_blocks(q, m, 16, 20, is_causal=False)
+    assert torch.equal(got.cpu(), so.select(q, m, 16, 20, False)[0])
+
+
+def test_select_close_scores():
+    """Scores a float32 sum cannot tell apart: means that differ in their last place."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(5)
+    base = _normal(gen, 1, 1, 1, 64)
+    m = base.expand(1, 200, 1, 64).clone()
+    step = torch.randint(-3, 4, m.shape, generator=gen, device="cuda")
+    m = (m.view(torch.int32) + step.int()).view(torch.float32)
+    q = _normal(gen, 1, 50, 2, 64)
+    got = jm.select_blocks(q, m, 16, 11, is_causal=False)
+    assert torch.equal(got.cpu(), so.select(q, m, 16, 11, False)[0])
+
+
+def test_select_views():
+    import jaxmodules_amd as jm
+
+    gen = _gen(6)
+    q, m = _normal(gen, 2, 4, 50, 64, dtype="bfloat16").transpose(1, 2), _normal(gen, 2, 2, 40, 64).transpose(1, 2)
+    odd = _normal(gen, 2 * 50 * 4 * 64 + 1, dtype="bfloat16")[1:].view(2, 50, 4, 64)
+    for x in (q, odd):
+        assert torch.equal(jm.select_blocks(x, m, 16, 5), jm.select_blocks(x.contiguous().clone(), m.contiguous(), 16, 5))
+
+
+# ---- attention -------------------------------------------------------------------------
+
+
+def _blocks(gen, B, N, Hkv, count, nblk):
+    """Any order, some of them past the query, repeated or -1."""
+    return torch.randint(-1, nblk + 1, (B, N, Hkv, count), generator=gen, device="cuda", dtype=torch.int32)
+
+
+def _check(got, want, dt, top, d, terms, what):
+    value, mag = want
+    tol = so.tolerance(value, mag, dt, top, d, terms)
+    err = (got.detach().cpu().double() - value).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((err / tol)[bad].max()))
+
+
+SHAPES = [
+    # B, N, L, Hq, Hkv, d, bs, count
+    (1, 1, 1, 1, 1, 8, 16, 1), (2, 40, 40, 4, 2, 64, 16, 3), (1, 300, 300, 8, 2, 64, 64, 3), (2, 129, 260, 6, 6, 128, 32, 5),
+    (1, 700, 700, 4, 1, 128, 64, 6), (1, 200, 500, 3, 1, 80, 128, 3), (1, 150, 600, 2, 2, 64, 256, 2),
+    (2, 60, 100, 40, 2, 64, 16, 4), (1, 400, 400, 2, 1, 40, 48, 40), (1, 90, 333, 4, 2, 20, 80, 3), (1, 2300, 260, 2, 1, 64, 64, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention(shape, causal, dtype):
+    import jaxmodules_amd as jm
+
+    B, N, L, Hq, Hkv, d, bs, count = shape
+    gen = _gen(N + L + d)
+    f = d ** -0.25
+    q, k, v = (_normal(gen, B, n, h, d, dtype=dtype, f=f).requires_grad_() for n, h in ((N, Hq), (L, Hkv), (L, Hkv)))
+    do = _normal(gen, B, N, Hq, d, dtype=dtype)
+    blocks = _blocks(gen, B, N, Hkv, count, -(-L // bs))
+    o = jm.selected_attention(q, k, v, blocks, bs, is_causal=causal)
+    assert o.dtype == q.dtype and o.shape == q.shape
+    with torch.no_grad():
+        assert torch.equal(o, jm.selected_attention(q, k, v, blocks, bs, is_causal=causal))
+    ok = so.visible(blocks, N, L, bs, causal, None, None)
+    want, top = so.attend(q, k, v, ok, do=do)
+    _check(o, want["o"], o.dtype, top, d, count * bs, "o")
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    for n, g in zip(("dq", "dk", "dv"), grads):
+        _check(g, want[n], o.dtype, top, d, max(count * bs, N * Hq // Hkv), n)
+    unseen = ~ok.any(2).permute(0, 2, 1)  # [B, L, Hkv]
+    assert not grads[1].cpu()[unseen].any() and not grads[2].cpu()[unseen].any()
+    empty = ~ok.any(3).permute(0, 2, 1).repeat_interleave(Hq // Hkv, 2)
+    assert not o.detach().cpu()[empty].any() and not grads[0].cpu()[empty].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("N,Hq,bs,count", [(1, 8, 64, 9), (1, 2, 16, 70), (4, 6, 32, 20), (17, 4, 64, 5), (1, 34, 128, 3)])
+def test_served_tokens(N, Hq, bs, count, dtype):
+    """The last tokens of ragged sequences in a cache whose unused rest holds NaN."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(N + Hq)
+    B, L, Hkv, d = 6, 1500, 2, 64
+    lengths = _ints(1500, 777, 64, max(N, 17), 1, 0)
+    starts = lengths - N
+    q = _normal(gen, B, N, Hq, d, dtype=dtype)
+    k, v = (_normal(gen, B, L, Hkv, d, dtype=dtype) for _ in range(2))
+    for b, n in enumerate(lengths.tolist()):
+        k[b, n:], v[b, n:] = float("nan"), float("nan")
+    blocks = _blocks(gen, B, N, Hkv, count, -(-L // bs))
+    for st in (starts, None):
+        causal = st is not None
+        o = jm.selected_attention(q, k, v, blocks, bs, starts=st, lengths=lengths, is_causal=causal)
+        want, top = so.attend(q, k, v, so.visible(blocks, N, L, bs, causal, st, lengths))
+        _check(o, want["o"], o.dtype, top, d, count * bs, "o")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("bs", [32, 128])
+def test_odd_values_stay_with_the_queries_that_see_them(dtype, bs):
+    """NaN and infinities in a token reach no query before it, in any output."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(8)
+    N = 200
+    q, k, v, do = (_normal(gen, 1, N, h, 64, dtype=dtype) for h in (4, 2, 2, 4))
+    blocks = torch.arange(-(-N // bs), device="cuda", dtype=torch.int32).expand(1, N, 2, -1).contiguous()
+
+    def grads(q, k, v, do):
+        x = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = jm.selected_attention(*x, blocks, bs)
+        return [o.detach(), *torch.autograd.grad(o, x, do)]
+
+    clean = grads(q, k, v, do)
+    at = 150
+    for which in range(4):
+        x = [t.clone() for t in (q, k, v, do)]
+        x[which][0, at, 0, 3], x[which][0, at, 0, 5] = float("nan"), float("inf")
+        got = grads(*x)
+        assert torch.equal(got[0][0, :at], clean[0][0, :at]) and torch.equal(got[1][0, :at], clean[1][0, :at]), which
+        # keys behind the token are not seen by it: an odd query or gradient does not reach them
+        if which in (0, 3):
+            for g, c in zip(got[2:], clean[2:]):
+                assert g[0, at + 1:].isfinite().all()
+                torch.testing.assert_close(g[0, at + 1:], c[0, at + 1:], rtol=2e-2, atol=1e-5)
+        assert not got[0 if which < 3 else 1][0, at].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_odd_values_reach_their_own_columns_alone(dtype, d):
+    """NaN and infinities in columns of one value (or key, query, gradient) leave the other
+    columns of every output that adds it as they are, and are seen in their own."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(15)
+    N, at, bs = 130, 70, 64
+    q, k, v, do = (_normal(gen, 1, N, 2, d, dtype=dtype) for _ in range(4))
+    blocks = torch.arange(3, device="cuda", dtype=torch.int32).expand(1, N, 2, -1).contiguous()
+    odd, cols = [3, d - 9], [c for c in range(d) if c not in (3, d - 9)]
+
+    def outputs(v, do):
+        x = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = jm.selected_attention(*x, blocks, bs)
+        return o.detach(), *torch.autograd.grad(o, x, do)
+
+    clean = outputs(v, do)
+    w = v.clone()
+    w[0, at, 0, odd[0]], w[0, at, 0, odd[1]] = float("nan"), float("inf")
+    o = outputs(w, do)[0]
+    assert torch.equal(o[..., cols], clean[0][..., cols]) and torch.equal(o[:, :at], clean[0][:, :at])
+    assert o[0, at:, 0, odd[0]].isnan().all() and (o[0, at:, 0, odd[1]] == float("inf")).all()
+    assert torch.equal(o[:, :, 1], clean[0][:, :, 1])
+    w = do.clone()
+    w[0, at, 0, odd[0]] = float("nan")
+    dv = outputs(v, w)[3]
+    assert torch.equal(dv[..., cols], clean[3][..., cols]) and torch.equal(dv[:, at + 1:], clean[3][:, at + 1:])
+    assert dv[0, : at + 1, 0, odd[0]].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_strides_scale_and_order(dtype):
+    import jaxmodules_amd as jm
+
+    gen = _gen(9)
+    B, N, H, d, bs = 2, 100, 2, 64, 32
+    heads_major = [_normal(gen, B, H, N, d, dtype=dtype).transpose(1, 2) for _ in range(3)]
+    flat = _normal(gen, B * N * H * d + 1, dtype=dtype)
+    odd = [flat[1:].view(B, N, H, d)] * 3
+    one = [_normal(gen, B, N, 1, d, dtype=dtype).expand(B, N, H, d)] * 3
+    blocks = _blocks(gen, B, N, H, 3, 4)
+    for views in (heads_major, odd, one):
+        for scale in (None, -0.3, 0.0):
+            res = []
+            for fit in (lambda t: t.detach(), lambda t: t.detach().clone(memory_format=torch.contiguous_format)):
+                x = [fit(t).requires_grad_() for t in views]
+                o = jm.selected_attention(*x, blocks if len(res) == 0 else blocks.flip(3).contiguous(), bs, scale=scale)
+                up = torch.ones(1, 1, 1, 1, dtype=o.dtype, device="cuda").expand_as(o)
+                res.append([o.detach(), *torch.autograd.grad(o, x, up)])
+            for a, b in zip(*res):  # (the order of the slots is the order of the sums)
+                torch.testing.assert_close(a, b, rtol=2 ** -6 if dtype == "bfloat16" else 1e-4, atol=2e-2 if dtype == "bfloat16" else 1e-5)
+            want, top = so.attend(*views, so.visible(blocks, N, N, bs, True, None, None), scale=0.125 if scale is None else scale)
+            _check(res[0][0], want["o"], res[0][0].dtype, top, d, 96, "o")
+
+
+def test_nothing_to_attend_to():
+    import jaxmodules_amd as jm
+
+    for shape_q, shape_k, count in (((0, 4, 2, 64), (0, 4, 2, 64), 1), ((1, 0, 2, 64), (1, 4, 2, 64), 1), ((1, 4, 2, 64), (1, 0, 2, 64), 1),
+                                    ((1, 4, 2, 64), (1, 4, 2, 64), 0)):
+        q, k, v = (torch.randn(s, device="cuda", requires_grad=True) for s in (shape_q, shape_k, shape_k))
+        blocks = torch.zeros((*shape_q[:2], shape_k[2], count), dtype=torch.int32, device="cuda")
+        o = jm.selected_attention(q, k, v, blocks, 16)
+        assert o.shape == q.shape and not o.any()
+        assert all(not g.any() and g.shape == x.shape for g, x in zip(torch.autograd.grad(o, (q, k, v), torch.ones_like(o)), (q, k, v)))
+    q, k, v = (torch.randn(1, 20, 2, 64, device="cuda", requires_grad=True) for _ in range(3))
+    o = jm.selected_attention(q, k, v, torch.full((1, 20, 2, 3), -1, dtype=torch.int32, device="cuda"), 16)
+    assert not o.any() and all(not g.any() for g in torch.autograd.grad(o, (q, k, v), torch.ones_like(o)))
+
+
+def test_gradients_of_some_inputs():
+    import jaxmodules_amd as jm
+
+    gen = _gen(11)
+    q, k, v = (_normal(gen, 1, 50, 2, 64) for _ in range(3))
+    blocks = _blocks(gen, 1, 50, 2, 2, 4)
+    full = [x.clone().requires_grad_() for x in (q, k, v)]
+    want = torch.autograd.grad(jm.selected_attention(*full, blocks, 16).sum(), full)
+    for i in range(3):
+        x = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        assert torch.equal(torch.autograd.grad(jm.selected_attention(*x, blocks, 16).sum(), x[i])[0], want[i])
+
+
+def test_gradient_against_differences():
+    """Central differences of the entry point in float32: the third derivative's h^2 and
+    the values' u / h are both below 1e-2 of the gradient here."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(12)
+    x = [_normal(gen, 1, 48, h, 64, f=0.35).requires_grad_() for h in (4, 2, 2)]
+    blocks = _blocks(gen, 1, 48, 2, 2, 3)
+    u = _normal(gen, 1, 48, 4, 64)
+    loss = lambda *t: (jm.selected_attention(*t, blocks, 16).double() * u).sum()  # noqa: E731
+    g = torch.autograd.grad(loss(*x), x)
+    with torch.no_grad():
+        for _ in range(6):
+            a = [_normal(gen, *t.shape) for t in x]
+            h = 2.0 ** -6
+            num = (loss(*(t + h * b for t, b in zip(x, a))) - loss(*(t - h * b for t, b in zip(x, a)))) / (2 * h)
+            terms = [(y.double() * b) for y, b in zip(g, a)]
+            assert abs(num - sum(t.sum() for t in terms)) <= 1e-2 * math.sqrt(sum(t.square().sum().item() for t in terms))
+
+
+def test_run_together_on_a_side_stream_and_captured():
+    """norm_rotary -> block_means -> select_blocks -> selected_attention and its backward,
+    as a model's layer runs them; every replay of the captured step equals the eager one."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(13)
+    B, N, Hq, Hkv, d = 1, 300, 4, 2, 64
+    q, k, v, do = (_normal(gen, B, N, h, d, dtype="bfloat16") for h in (Hq, Hkv, Hkv, Hq))
+    w = torch.ones(d, device="cuda")
+    f, scale = jm.rotary_frequencies(d, device="cuda")
+
+    def step():
+        x = [t.detach().requires_grad_() for t in (q, k, v, w)]
+        a, c = jm.norm_rotary(x[0], x[1], x[3], x[3], inv_freq=f, scale=scale)
+        blocks = jm.select_blocks(a, jm.block_means(c, 32), 32, 4)
+        o = jm.selected_attention(a, c, x[2], blocks, 32)
+        return [blocks, o.detach(), *torch.autograd.grad(o, x, do)]
+
+    want = step()
+    ok = so.visible(want[0], N, N, 32, True, None, None)
+    a, c = jm.norm_rotary(q, k, w, w, inv_freq=f, scale=scale)
+    ref, top = so.attend(a, c, v, ok)
+    _check(want[1], ref["o"], torch.bfloat16, top, d, 128, "o")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    s.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(side, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        for t in (q, k, v):
+            t.copy_(torch.randn_like(t))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, eager)), i
+
+
+def test_a_token_served_equals_the_prompt():
+    """Each token of a sequence from a cache (means kept up, one query) gives what the
+    whole prompt gave for it."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(14)
+    L, bs, d = 150, 16, 64
+    q, k, v = (_normal(gen, 2, L, h, d) for h in (4, 2, 2))
+    blocks = jm.select_blocks(q, jm.block_means(k, bs), bs, 4)
+    prompt = jm.selected_attention(q, k, v, blocks, bs)
+    cache_k, cache_v = (torch.full_like(x, float("nan")) for x in (k, v))
+    means = torch.zeros((2, -(-L // bs), 2, d), device="cuda")
+    for t in range(L):
+        cache_k[:, t], cache_v[:, t] = k[:, t], v[:, t]
+        lengths = torch.full((2,), t + 1, dtype=torch.int32, device="cuda")
+        jm.block_means(cache_k, bs, lengths, out=means, new=1)
+        b = jm.select_blocks(q[:, t:t + 1], means, bs, 4, starts=lengths - 1, lengths=lengths)
+        assert torch.equal(b[:, 0], blocks[:, t]), t
+        o = jm.selected_attention(q[:, t:t + 1], cache_k, cache_v, b, bs, starts=lengths - 1, lengths=lengths)
+        torch.testing.assert_close(o[:, 0], prompt[:, t], rtol=1e-4, atol=1e-5)
+
+
+def test_blocks_changed_before_the_backward_are_an_error():
+    import jaxmodules_amd as jm
+
+    x = [torch.randn(1, 40, 2, 64, device="cuda", requires_grad=True) for _ in range(3)]
+    blocks = torch.zeros((1, 40, 2, 1), dtype=torch.int32, device="cuda")
+    o = jm.selected_attention(*x, blocks, 16)
+    blocks.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
