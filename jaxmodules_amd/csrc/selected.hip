@@ -33,6 +33,8 @@ namespace {
 
 constexpr int kChunkQ = 256;    // queries a list workgroup takes
 constexpr int kRange = 1024;    // blocks a list workgroup takes
+constexpr int kSlotBits = 10;   // of a list entry
+constexpr int kMaxSel = 1 << kSlotBits;  // blocks of a query
 constexpr int kRows = 512;      // rows (query, head) of a block that a forward or dQ workgroup takes
 constexpr int kRowsKV = 2048;   // rows that a dK/dV workgroup takes
 
@@ -55,7 +57,7 @@ struct SArgs {
   int* cnt;                  // [B * Hkv][nblk][chunks]: entries of a chunk, then their first index in the block's list
   int* off;                  // [B * Hkv][nblk + 1]
   int* kvoff;                // [B * Hkv][nblk + 1]: first dK/dV item of a block
-  int* ent;                  // [B * Hkv][Lq * count]: query * count + slot, by block, in the order of queries
+  int* ent;                  // [B * Hkv][Lq * count]: (query << kSlotBits) + slot, by block, in the order of queries
   Desc *tile, *kvtile;       // [B * Hkv][max_tiles], [B * Hkv][max_kv]
   int words, chunks, max_tiles, max_kv, subs;  // subs: dK/dV key tiles of a block
 };
@@ -122,7 +124,7 @@ void list_entries(SArgs a) {
         int r = __popc(bits[j][t >> 5] & (mine - 1));
         for (int x = 0; x < (t >> 5); ++x) r += __popc(bits[j][x]);
         a.ent[(int64_t)bh * p.Lq * p.count + a.off[(int64_t)bh * (a.nblk + 1) + lo + j] +
-              a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] + r] = q * p.count + c;
+              a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] + r] = (q << kSlotBits) + c;
       }
     }
   }
@@ -220,8 +222,8 @@ struct RowId {
   int q, slot, g;
 };
 __device__ __forceinline__ RowId row_id(const SArgs& a, const int* list, int r) {
-  const int e = r / a.G, x = list[e], q = x / a.p.count;
-  return RowId{q, x - q * a.p.count, r - e * a.G};
+  const int e = r / a.G, x = list[e];
+  return RowId{x >> kSlotBits, x & ((1 << kSlotBits) - 1), r - e * a.G};
 }
 
 // Rows k0 .. k0 + N - 1 of a [L, D] slice to LDS, zeros for rows at or past `end` and columns
@@ -287,7 +289,7 @@ constexpr int kKT = 64;  // keys of a staged tile
 // P and dS are rounded to the inputs' type (as V and K are), sums are float32; the sum of
 // the weights adds them as rounded, so that O is a weighted mean of V's rows.
 template <class Tag, int D, bool GRAD>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(SOp<Tag>::ES == 2 && (D == 64 || !GRAD) ? 2 : 1)))
 void by_block_q(SArgs a) {
   using O = SOp<Tag>;
   using T = STile<Tag, D>;
@@ -309,20 +311,31 @@ void by_block_q(SArgs a) {
   char *kt = lds, *vt = lds + kKT * T::RB;
   bool odd = false;  // GRAD: the tile of K holds an infinite or NaN value
 
-  for (int r0 = 0; r0 < rows; r0 += 128) {
-    const int r = r0 + 32 * wave + l32;
-    const bool live = r < rows;
-    const RowId id = row_id(a, list, desc.row0 + min(r, rows - 1));
-    const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
-    const int h = hk * a.G + id.g;
-    typename O::Frag qf[D / 16], gf[GRAD ? D / 16 : 1];
-    load_rows<Tag, D>(qf, a.q, b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2], hi, p.D);
-    float lse = 0.f, delta = 0.f;
+  // a row's operands; those of the next 128 rows are loaded ahead of the products of these
+  struct Rows {
+    RowId id;
+    typename O::Frag q[D / 16], g[GRAD ? D / 16 : 1];
+    float lse, delta;
+  };
+  const auto load = [&](Rows& x, int r0) {
+    x.id = row_id(a, list, desc.row0 + min(r0 + 32 * wave + l32, rows - 1));
+    const int h = hk * a.G + x.id.g;
+    load_rows<Tag, D>(x.q, a.q, b * p.q_stride[0] + x.id.q * p.q_stride[1] + h * p.q_stride[2], hi, p.D);
     if constexpr (GRAD) {
-      load_rows<Tag, D>(gf, a.dO, b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2], hi, p.D);
-      lse = a.lse[row];
-      delta = a.delta[row];
+      const int64_t row = ((int64_t)bh * p.Lq + x.id.q) * a.G + x.id.g;
+      load_rows<Tag, D>(x.g, a.dO, b * p.do_stride[0] + x.id.q * p.do_stride[1] + h * p.do_stride[2], hi, p.D);
+      x.lse = a.lse[row];
+      x.delta = a.delta[row];
     }
+  };
+  Rows next;
+  load(next, 0);
+  for (int r0 = 0; r0 < rows; r0 += 128) {
+    const bool live = r0 + 32 * wave + l32 < rows;
+    const Rows now = next;
+    const RowId id = now.id;
+    if (r0 + 128 < rows) load(next, r0 + 128);
+    const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
     const int64_t lim = key_limit(p, b, id.q, held, start) - k0;  // keys of the block the row sees
     const int see = (int)min(lim, (int64_t)inside);
     f32x16 acc[D / 32];
@@ -340,36 +353,41 @@ void by_block_q(SArgs a) {
         else __syncthreads();
       }
       const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
-      // (single floats from here on: of a 16-register result changed in a branch the compiler
-      // has written back registers of another value)
-      float s[2][16];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      // S^T of 32 keys: single floats from here on (of a 16-register result changed in a branch
+      // the compiler has written back registers of another value)
+      const auto scores = [&](const char* t, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
         f32x16 r16 = f32x16{};
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(kt, 32 * x + l32, 2 * c + hi), qf[c], r16);
+        for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(t, 32 * x + l32, 2 * c + hi), f[c], r16);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = r16[i];
-      }
-      uint32_t vis[2] = {0xffffu, 0xffffu};
-      if (part) {
+        for (int i = 0; i < 16; ++i) s[i] = r16[i];
+      };
+      const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) vis[x] = below(see - t * kKT - 32 * x, hi);
-      }
+        for (int j = 0; j < 2; ++j) {
+          float e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = s[8 * j + i];
+          f[j] = O::pack(e);
+        }
+      };
       if constexpr (!GRAD) {
-        float top = NEG_INF;
+        float s[2][16], top = NEG_INF;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) scores(kt, now.q, x, s[x]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            s[x][i] = !part || ((vis[x] >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
+            s[x][i] = !part || ((vis >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
             top = fmaxf(top, s[x][i]);
           }
+        }
         top = fmaxf(m, wave_max32(top));
         const float ref = top == NEG_INF ? 0.f : top;
-        const float keep = fast_exp2(m - ref);
-        m = top;
         if (t > 0) {
+          const float keep = fast_exp2(m - ref);
           sum *= keep;
           exact *= keep;
 #pragma unroll
@@ -377,52 +395,51 @@ void by_block_q(SArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[mt][i] *= keep;
         }
+        m = top;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             s[x][i] = fast_exp2(s[x][i] - ref);
             exact += s[x][i];
           }
+          typename O::Frag f[2];
+          operands(s[x], f);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if constexpr (O::ES == 2) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
+            }
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * x + j, mt, lane), f[j], acc[mt]);
+          }
+        }
       } else {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          f32x16 dp = f32x16{};
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) dp = O::mma32(T::row(vt, 32 * x + l32, 2 * c + hi), gf[c], dp);
+          float s[16], dp[16];
+          scores(kt, now.q, x, s);
+          scores(vt, now.g, x, dp);
+          const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float w = fast_exp2(s[x][i] * a.scale_log2 - lse) * (dp[i] - delta);
-            s[x][i] = !part || ((vis[x] >> i) & 1u) ? w : 0.f;
+            const float w = fast_exp2(s[i] * a.scale_log2 - now.lse) * (dp[i] - now.delta);
+            s[i] = !part || ((vis >> i) & 1u) ? w : 0.f;
           }
-        }
-      }
-      // P^T V^T, or dS^T K^T
-      const char* xt = GRAD ? kt : vt;
+          typename O::Frag f[2];
+          operands(s, f);
+          if (odd) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        typename O::Frag f[2];
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float e[8];
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(kt, 2 * x + j, mt, lane)), f[j], acc[mt]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = s[x][8 * j + i];
-          f[j] = O::pack(e);
-          if constexpr (!GRAD && O::ES == 2) {
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(kt, 2 * x + j, mt, lane), f[j], acc[mt]);
           }
-        }
-        if (GRAD && odd) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(xt, 2 * x + j, mt, lane)), f[j], acc[mt]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(xt, 2 * x + j, mt, lane), f[j], acc[mt]);
         }
       }
     }
@@ -454,6 +471,9 @@ void by_block_kv(SArgs a) {
   __shared__ __align__(16) char lds[2 * NR * T::RB];
   __shared__ __align__(16) float s_lse[NR], s_delta[NR];
   __shared__ __align__(16) int s_see[NR];
+  __shared__ int64_t s_q[NR], s_g[NR];
+  float n_lse = 0.f, n_delta = 0.f;
+  int n_see = 0;
   const mattn_selected& p = a.p;
   const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
   const int64_t item = (int64_t)bh * a.max_kv + blockIdx.x / a.bh_n;
@@ -484,36 +504,53 @@ void by_block_kv(SArgs a) {
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) dk[mt] = dv[mt] = f32x16{};
 
-  for (int r0 = 0; r0 < rows; r0 += NR) {
-    __syncthreads();
-    constexpr int EC = 16 / O::ES, TPR = T::CPR < 16 ? T::CPR : 16;  // threads of a row
-#pragma unroll
-    for (int i = 0; i < NR * TPR / 256; ++i) {
-      const int x = i * 256 + threadIdx.x, r = x / TPR;
+  // rows of the next stage: where they are (ids), then their values (rq, rg in registers)
+  // while this stage's products run
+  constexpr int EC = 16 / O::ES, N = NR * T::CPR / 256;  // chunks of a thread
+  const auto ids = [&](int r0) {
+    if (threadIdx.x < NR) {
+      const int r = threadIdx.x;
       const bool live = r0 + r < rows;
       const RowId id = row_id(a, list, row0 + min(r0 + r, rows - 1));
       const int h = hk * a.G + id.g;
-      const char* qp = (const char*)a.q + O::ES * (b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2]);
-      const char* gp = (const char*)a.dO + O::ES * (b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2]);
-#pragma unroll
-      for (int ci = 0; ci < T::CPR / TPR; ++ci) {
-        const int c = x % TPR + ci * TPR;
-        u32x4 u = {0u, 0u, 0u, 0u}, w = {0u, 0u, 0u, 0u};
-        if (live && c * EC < p.D) {
-          u = *(const u32x4*)(qp + 16 * c);
-          w = *(const u32x4*)(gp + 16 * c);
-        }
-        *(u32x4*)(qt + T::at(r, c)) = u;
-        *(u32x4*)(gt + T::at(r, c)) = w;
-      }
-      if (x % TPR == 0) {
-        const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
-        s_lse[r] = live ? a.lse[row] : 0.f;
-        s_delta[r] = live ? a.delta[row] : 0.f;
-        s_see[r] = live ? (int)min(max((int64_t)key_limit(p, b, id.q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
-      }
+      const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
+      s_q[r] = b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2];
+      s_g[r] = b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2];
+      n_lse = live ? a.lse[row] : 0.f;
+      n_delta = live ? a.delta[row] : 0.f;
+      n_see = live ? (int)min(max((int64_t)key_limit(p, b, id.q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
     }
+  };
+  u32x4 xq[N], xg[N];
+  const auto fetch = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
+      const bool live = r0 + r < rows && c * EC < p.D;
+      xq[i] = live ? *(const u32x4*)((const char*)a.q + O::ES * (s_q[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
+      xg[i] = live ? *(const u32x4*)((const char*)a.dO + O::ES * (s_g[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  ids(0);
+  __syncthreads();
+  fetch(0);
+  for (int r0 = 0; r0 < rows; r0 += NR) {
+    __syncthreads();  // the stage before is done with the tiles, all have read the ids
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
+      *(u32x4*)(qt + T::at(r, c)) = xq[i];
+      *(u32x4*)(gt + T::at(r, c)) = xg[i];
+    }
+    if (threadIdx.x < NR) {
+      s_lse[threadIdx.x] = n_lse;
+      s_delta[threadIdx.x] = n_delta;
+      s_see[threadIdx.x] = n_see;
+    }
+    const bool more = r0 + NR < rows;
+    if (more) ids(r0 + NR);
     __syncthreads();
+    if (more) fetch(r0 + NR);
 #pragma unroll
     for (int i32 = 0; i32 < NR / 32 / RG; ++i32) {
       const int x = rg + i32 * RG;
@@ -623,7 +660,7 @@ __device__ __forceinline__ bool group_any(bool x, int lpr) {
 // What the infinite and NaN values of a block's V (GRAD: K) give to a row's O (dQ), which
 // lpr lanes hold 4 columns each: weights from the formula, the row's lse known.
 template <class Tag, bool GRAD>
-__device__ __noinline__ void add_odd_keys(const SArgs& a, f32x4& o, float lse, int64_t row, int b, int hk, int h, int q, int blk,
+__device__ __forceinline__ void add_odd_keys(const SArgs& a, f32x4& o, float lse, int64_t row, int b, int hk, int h, int q, int blk,
                                           int col, int lpr) {
   const mattn_selected& p = a.p;
   const int held = keys_held(p, b), lim = key_limit(p, b, q, held, first_pos(p, b));
@@ -661,7 +698,7 @@ __device__ __noinline__ void add_odd_keys(const SArgs& a, f32x4& o, float lse, i
 
 // The same of the rows of a block's list for 4 columns of a key's dK (W = 0) or dV (W = 1).
 template <class Tag, int W>
-__device__ __noinline__ void add_odd_rows(const SArgs& a, float (&o)[4], int bh, int key, int blk, int col) {
+__device__ __forceinline__ void add_odd_rows(const SArgs& a, float (&o)[4], int bh, int key, int blk, int col) {
   const mattn_selected& p = a.p;
   const int b = bh / p.Hkv, hk = bh % p.Hkv, held = keys_held(p, b);
   const int* off = a.off + (int64_t)bh * (a.nblk + 1) + blk;
@@ -710,42 +747,48 @@ void join_rows(SArgs a, int lpr_log2, int slots, bool all) {
   const float* plse = a.plse + row * slots;
   const auto valid = [&](int s) { return all || ((ok[s >> 5] >> (s & 31)) & 1u); };
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float lse = GRAD ? a.lse[row] : NEG_INF;
+  float lse = GRAD ? a.lse[row] : NEG_INF, sum = 0.f, m = NEG_INF;
+  // weights of the slots, lpr at a time, a lane each
   if constexpr (!GRAD) {
-    float m = NEG_INF;
     bool nan = false;
-    for (int s = 0; s < slots; ++s)
+    for (int s = lane; s < slots; s += lpr)
       if (valid(s)) {
         m = fmaxf(m, plse[s]);
         nan = nan || plse[s] != plse[s];
       }
-    if (nan) m = __builtin_nanf("");
-    float sum = 0.f;
-    if (m != NEG_INF) {
-#pragma unroll 4
-      for (int s = 0; s < slots; ++s) {
-        if (!valid(s)) continue;
-        const float w = fast_exp2(plse[s] - m);
-        if (w == 0.f) continue;
-        sum += w;
-        if (col < p.D) {
-          const f32x4 x = *(const f32x4*)(part + (int64_t)s * p.D + col);
+    for (int d = lpr >> 1; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (group_any(nan, lpr)) m = __builtin_nanf("");
+  }
+  if (GRAD || m != NEG_INF) {
+    for (int s0 = 0; s0 < slots; s0 += lpr) {
+      const int s = s0 + lane;
+      float w = 0.f;
+      if (s < slots && valid(s)) w = GRAD ? 1.f : fast_exp2(plse[s] - m);
+      sum += w;
+      const int n = min(lpr, slots - s0);
+      for (int i = 0; i < n; i += 8) {  // 8 rows in flight; unused slots are read, not added
+        f32x4 x[8];
+        float y[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] += w * x[i];
+        for (int e = 0; e < 8; ++e) {
+          y[e] = __shfl(w, (threadIdx.x & 63 & ~(lpr - 1)) + min(i + e, lpr - 1));
+          if (i + e >= n) y[e] = 0.f;
+          x[e] = *(const f32x4*)(part + (int64_t)min(s0 + i + e, slots - 1) * p.D + min(col, p.D - 4));
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] += y[e] != 0.f ? y[e] * x[e][c] : 0.f;
       }
+    }
+  }
+  if constexpr (!GRAD) {
+    for (int d = lpr >> 1; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (m != NEG_INF) {
       const float r = 1.f / sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= r;
+      for (int c = 0; c < 4; ++c) o[c] *= r;
       lse = m + __log2f(sum);
-    }
-  } else if (col < p.D) {
-#pragma unroll 4
-    for (int s = 0; s < slots; ++s) {
-      if (!valid(s)) continue;
-      const f32x4 x = *(const f32x4*)(part + (int64_t)s * p.D + col);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += x[i];
     }
   }
   const int b = bh / p.Hkv, h = bh % p.Hkv * a.G + g;
@@ -832,7 +875,6 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-constexpr int kMaxSel = 1024;  // blocks of a query
 template <class Tag, int D>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
 void by_query(SArgs a, int splits, int hgroups) {
@@ -1045,7 +1087,7 @@ int sel_check(const mattn_selected* p) {
     for (int i = 0; i < 3; ++i)
       if (s[i] < 0 || (s[i] * es) % 16) return MATTN_ERR_STRIDE;
   const int64_t lim = 1ll << 31, bh = (int64_t)p->B * p->Hkv, G = p->Hq / p->Hkv;
-  if (p->Lk + (int64_t)p->block_size >= lim || (int64_t)p->Lq * p->count * G >= lim || bh > 32767 || bh * p->Lq * G >= lim / 64)
+  if (p->Lk + (int64_t)p->block_size >= lim || p->Lq >= lim >> kSlotBits || (int64_t)p->Lq * p->count * G >= lim || bh > 32767 || bh * p->Lq * G >= lim / 64)
     return MATTN_ERR_TOO_LARGE;
   return MATTN_OK;
 }
