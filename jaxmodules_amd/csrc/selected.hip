@@ -58,6 +58,8 @@ struct SArgs {
   int* off;                  // [B * Hkv][nblk + 1]
   int* kvoff;                // [B * Hkv][nblk + 1]: first dK/dV item of a block
   int* ent;                  // [B * Hkv][Lq * count]: (query << kSlotBits) + slot, by block, in the order of queries
+  int* pos;                  // [B * Hkv][Lq * count]: index in ent of each query's slots that count
+  void* ds;                  // [B * Hkv][Lq * count (as ent)][G][block_size] dS / scale, the inputs' type (or null)
   Desc *tile, *kvtile;       // [B * Hkv][max_tiles], [B * Hkv][max_kv]
   int words, chunks, max_tiles, max_kv, subs;  // subs: dK/dV key tiles of a block
 };
@@ -123,8 +125,10 @@ void list_entries(SArgs a) {
         if (j < 0 || j >= n) continue;
         int r = __popc(bits[j][t >> 5] & (mine - 1));
         for (int x = 0; x < (t >> 5); ++x) r += __popc(bits[j][x]);
-        a.ent[(int64_t)bh * p.Lq * p.count + a.off[(int64_t)bh * (a.nblk + 1) + lo + j] +
-              a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] + r] = (q << kSlotBits) + c;
+        const int64_t head = (int64_t)bh * p.Lq * p.count;
+        const int at = a.off[(int64_t)bh * (a.nblk + 1) + lo + j] + a.cnt[((int64_t)bh * a.nblk + lo + j) * a.chunks + chunk] + r;
+        a.ent[head + at] = (q << kSlotBits) + c;
+        a.pos[head + (int64_t)q * p.count + c] = at;
       }
     }
   }
@@ -280,6 +284,14 @@ __device__ __forceinline__ uint32_t below(int lim, int hi) {
   return m;
 }
 
+// Bit i of vis as all ones or zero, opaque to the compiler (which would make it a compare
+// and a select): masking an element is then one bit operation.
+__device__ __forceinline__ uint32_t seen_bit(uint32_t vis, int i) {
+  uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)vis, i, 1);
+  asm("" : "+v"(m));
+  return m;
+}
+
 constexpr int kKT = 64;  // keys of a staged tile
 
 // Forward and dQ.  Four waves of 32 rows each (lane = row, both halves of a wave), 128 rows
@@ -309,7 +321,7 @@ void by_block_q(SArgs a) {
   const char* kb = (const char*)a.k + O::ES * (b * p.k_stride[0] + hk * p.k_stride[2]);
   const char* vb = (const char*)a.v + O::ES * (b * p.v_stride[0] + hk * p.v_stride[2]);
   char *kt = lds, *vt = lds + kKT * T::RB;
-  bool odd = false;  // GRAD: the tile of K holds an infinite or NaN value
+  bool odd = false;  // GRAD: some tile of K holds an infinite or NaN value
 
   // a row's operands; those of the next 128 rows are loaded ahead of the products of these
   struct Rows {
@@ -339,17 +351,18 @@ void by_block_q(SArgs a) {
     const int64_t lim = key_limit(p, b, id.q, held, start) - k0;  // keys of the block the row sees
     const int see = (int)min(lim, (int64_t)inside);
     f32x16 acc[D / 32];
+    float m, sum, exact;
+    const auto walk = [&](auto careful) {
 #pragma unroll
     for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
-    float m = NEG_INF, sum = 0.f, exact = 0.f;
-
+    m = NEG_INF, sum = exact = 0.f;
     for (int t = 0; t < tiles; ++t) {
-      if (tiles > 1 || r0 == 0) {
+      if (tiles > 1 || (r0 == 0 && !decltype(careful)::value)) {
         __syncthreads();
         const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
         const bool vo = stage_keys<Tag, D, kKT, !GRAD>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
         if (GRAD ? ko : vo) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
-        if constexpr (GRAD) odd = __syncthreads_or(ko);
+        if constexpr (GRAD) odd = __syncthreads_or(ko) || odd;
         else __syncthreads();
       }
       const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
@@ -429,19 +442,21 @@ void by_block_q(SArgs a) {
           }
           typename O::Frag f[2];
           operands(s, f);
-          if (odd) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(kt, 2 * x + j, mt, lane)), f[j], acc[mt]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(kt, 2 * x + j, mt, lane), f[j], acc[mt]);
-          }
+            for (int mt = 0; mt < D / 32; ++mt) {
+              auto y = T::tr32(kt, 2 * x + j, mt, lane);
+              if constexpr (decltype(careful)::value) y = O::finite(y);
+              acc[mt] = O::mma32(y, f[j], acc[mt]);
+            }
         }
       }
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (GRAD) {
+      if (odd) walk(std::true_type{});
     }
     const int64_t out = row * p.count + id.slot;
     if constexpr (GRAD) {
@@ -462,7 +477,8 @@ void by_block_q(SArgs a) {
 // registers and, with KT = 64, every other 32 rows; the scores' result has the rows along
 // its registers, so P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they
 // stand.  Float32 partial sums per item; the items of a block are added in order.
-template <class Tag, int D, int KT>
+// DS: dS also goes to memory, rows of block_size keys in the order of the list, through LDS.
+template <class Tag, int D, int KT, bool DS>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
 void by_block_kv(SArgs a) {
   using O = SOp<Tag>;
@@ -472,8 +488,8 @@ void by_block_kv(SArgs a) {
   __shared__ __align__(16) float s_lse[NR], s_delta[NR];
   __shared__ __align__(16) int s_see[NR];
   __shared__ int64_t s_q[NR], s_g[NR];
-  float n_lse = 0.f, n_delta = 0.f;
-  int n_see = 0;
+  constexpr int DSB = KT * O::ES + 16;  // bytes of a staged row of dS (16 more: rows start on other banks)
+  __shared__ __align__(16) char s_ds[DS ? NR * DSB : 16];
   const mattn_selected& p = a.p;
   const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
   const int64_t item = (int64_t)bh * a.max_kv + blockIdx.x / a.bh_n;
@@ -501,61 +517,76 @@ void by_block_kv(SArgs a) {
     for (int c = 0; c < D / 16; ++c) kf[c] = vf[c] = O::zero();
   }
   f32x16 dk[D / 32], dv[D / 32];
-#pragma unroll
-  for (int mt = 0; mt < D / 32; ++mt) dk[mt] = dv[mt] = f32x16{};
 
-  // rows of the next stage: where they are (ids), then their values (rq, rg in registers)
-  // while this stage's products run
+  // Rows come from all over memory, microseconds away: those of the next stage are on
+  // their way while this stage's products run.  Per stage: the list's entries (a stage before),
+  // where the rows lie (ids, in LDS), their values (fetch, in registers).
   constexpr int EC = 16 / O::ES, N = NR * T::CPR / 256;  // chunks of a thread
-  const auto ids = [&](int r0) {
-    if (threadIdx.x < NR) {
-      const int r = threadIdx.x;
-      const bool live = r0 + r < rows;
-      const RowId id = row_id(a, list, row0 + min(r0 + r, rows - 1));
-      const int h = hk * a.G + id.g;
-      const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
-      s_q[r] = b * p.q_stride[0] + id.q * p.q_stride[1] + h * p.q_stride[2];
-      s_g[r] = b * p.do_stride[0] + id.q * p.do_stride[1] + h * p.do_stride[2];
-      n_lse = live ? a.lse[row] : 0.f;
-      n_delta = live ? a.delta[row] : 0.f;
-      n_see = live ? (int)min(max((int64_t)key_limit(p, b, id.q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
-    }
+  struct Stage {
+    u32x4 q[N], g[N];
+    float lse, delta;
+    int see;
   };
-  u32x4 xq[N], xg[N];
-  const auto fetch = [&](int r0) {
+  int entry = 0;  // thread r < NR: of row r of the stage after the last one with ids
+  const auto look = [&](int r0) {
+    if (threadIdx.x < NR) entry = list[(row0 + min(r0 + (int)threadIdx.x, rows - 1)) / a.G];
+  };
+  const auto ids = [&](Stage& w, int r0) {
+    if (threadIdx.x < NR) {
+      const int r = threadIdx.x, q = entry >> kSlotBits, g = (row0 + min(r0 + r, rows - 1)) % a.G;
+      const bool live = r0 + r < rows;
+      const int h = hk * a.G + g;
+      const int64_t row = ((int64_t)bh * p.Lq + q) * a.G + g;
+      s_q[r] = b * p.q_stride[0] + q * p.q_stride[1] + h * p.q_stride[2];
+      s_g[r] = b * p.do_stride[0] + q * p.do_stride[1] + h * p.do_stride[2];
+      w.lse = a.lse[row];
+      w.delta = a.delta[row];
+      w.see = live ? (int)min(max((int64_t)key_limit(p, b, q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
+    }
+    look(r0 + NR);
+  };
+  const auto fetch = [&](Stage& w, int r0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
       const bool live = r0 + r < rows && c * EC < p.D;
-      xq[i] = live ? *(const u32x4*)((const char*)a.q + O::ES * (s_q[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
-      xg[i] = live ? *(const u32x4*)((const char*)a.dO + O::ES * (s_g[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
+      w.q[i] = live ? *(const u32x4*)((const char*)a.q + O::ES * (s_q[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
+      w.g[i] = live ? *(const u32x4*)((const char*)a.dO + O::ES * (s_g[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
     }
   };
-  ids(0);
-  __syncthreads();
-  fetch(0);
-  for (int r0 = 0; r0 < rows; r0 += NR) {
-    __syncthreads();  // the stage before is done with the tiles, all have read the ids
+  const auto put_ds = [&](int r0) {  // rows r0 .. r0 + NR - 1
+    if constexpr (DS) {
+      const int keys = min(KT, p.block_size - sub * KT) * O::ES / 16;  // chunks of a row
+      char* o = (char*)a.ds + O::ES * ((((int64_t)bh * p.Lq * p.count + off[0]) * a.G + row0 + r0) * p.block_size + sub * KT);
+#pragma unroll
+      for (int i = 0; i < NR * (KT * O::ES / 16) / 256; ++i) {
+        const int x = i * 256 + threadIdx.x, r = x / (KT * O::ES / 16), c = x % (KT * O::ES / 16);
+        if (r0 + r < rows && c < keys) *(u32x4*)(o + (int64_t)r * p.block_size * O::ES + 16 * c) = *(const u32x4*)(s_ds + r * DSB + 16 * c);
+      }
+    }
+  };
+  const auto stage = [&](Stage& w, int r0, auto careful) {
+    barrier_lds();  // the stage before is done with the tiles, all have read the ids
+    if (r0 > 0) put_ds(r0 - NR);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
-      *(u32x4*)(qt + T::at(r, c)) = xq[i];
-      *(u32x4*)(gt + T::at(r, c)) = xg[i];
+      *(u32x4*)(qt + T::at(r, c)) = w.q[i];
+      *(u32x4*)(gt + T::at(r, c)) = w.g[i];
     }
     if (threadIdx.x < NR) {
-      s_lse[threadIdx.x] = n_lse;
-      s_delta[threadIdx.x] = n_delta;
-      s_see[threadIdx.x] = n_see;
+      s_lse[threadIdx.x] = w.lse;
+      s_delta[threadIdx.x] = w.delta;
+      s_see[threadIdx.x] = w.see;
     }
     const bool more = r0 + NR < rows;
-    if (more) ids(r0 + NR);
-    __syncthreads();
-    if (more) fetch(r0 + NR);
+    if (more) ids(w, r0 + NR);
+    barrier_lds();
+    if (more) fetch(w, r0 + NR);
 #pragma unroll
     for (int i32 = 0; i32 < NR / 32 / RG; ++i32) {
       const int x = rg + i32 * RG;
       if (r0 + 32 * x >= rows) continue;
-      uint32_t vis = 0u;
       float s[16], dp[16];
       {
         f32x16 x16 = f32x16{}, y16 = f32x16{};
@@ -563,23 +594,36 @@ void by_block_kv(SArgs a) {
         for (int c = 0; c < D / 16; ++c) x16 = O::mma32(T::row(qt, 32 * x + l32, 2 * c + hi), kf[c], x16);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) y16 = O::mma32(T::row(gt, 32 * x + l32, 2 * c + hi), vf[c], y16);
+        if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 4, 1>();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[i] = x16[i];
           dp[i] = y16[i];
         }
       }
+      const bool part = __any(s_see[32 * x + l32] < KT);  // some row does not see all of the tile
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 32 * x + 8 * j + 4 * hi;
         const f32x4 l = *(const f32x4*)(s_lse + r), d = *(const f32x4*)(s_delta + r);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool see = key < s_see[r + i];
-          vis |= (uint32_t)see << (4 * j + i);
-          const float w = fast_exp2(s[4 * j + i] * a.scale_log2 - l[i]);
-          s[4 * j + i] = see ? w : 0.f;
-          dp[4 * j + i] = see ? w * (dp[4 * j + i] - d[i]) : 0.f;
+          const float w = fast_exp2(__builtin_fmaf(s[4 * j + i], a.scale_log2, -l[i])), g = w * (dp[4 * j + i] - d[i]);
+          s[4 * j + i] = w;
+          dp[4 * j + i] = g;
+        }
+      }
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 n = *(const u32x4*)(s_see + 32 * x + 8 * j + 4 * hi);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t see = key < (int)n[i] ? 0xffffffffu : 0u;
+            asm("" : "+v"(see));
+            s[4 * j + i] = mask_zero(s[4 * j + i], see);
+            dp[4 * j + i] = mask_zero(dp[4 * j + i], see);
+          }
         }
       }
       typename O::Frag pf[2], df[2];
@@ -594,24 +638,54 @@ void by_block_kv(SArgs a) {
         pf[j] = O::pack(e);
         df[j] = O::pack(y);
       }
-      const bool part = __any(vis != 0xffffu);
-      const auto add = [&](f32x16(&acc)[D / 32], const char* t, const typename O::Frag(&f)[2]) {
-        if (part && T::odd(t + 32 * x * T::RB, 32, lane)) {
-          a.kvodd[(int64_t)bh * a.nblk + desc.blk] = 1;
+      if constexpr (DS) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(O::finite(T::tr32(t, 2 * x + j, mt, lane)), f[j], acc[mt]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(t, 2 * x + j, mt, lane), f[j], acc[mt]);
+        for (int i = 0; i < 16; ++i) {
+          char* at = s_ds + (32 * x + 8 * (i >> 2) + 4 * hi + (i & 3)) * DSB + key * O::ES;
+          if constexpr (O::ES == 4) *(float*)at = dp[i];
+          else *(uint16_t*)at = (uint16_t)elt16(__builtin_bit_cast(u32x4, df[i >> 3]), i & 7);
         }
+      }
+      const auto add = [&](f32x16(&acc)[D / 32], const char* t, const typename O::Frag(&f)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int mt = 0; mt < D / 32; ++mt) {
+            auto y = T::tr32(t, 2 * x + j, mt, lane);
+            if constexpr (decltype(careful)::value) y = O::finite(y);
+            acc[mt] = O::mma32(y, f[j], acc[mt]);
+          }
+        if constexpr (O::ES == 2) reads_ahead<2 * D / 32, 4, 2>();
       };
       add(dv, gt, pf);
       add(dk, qt, df);
     }
+  };
+  const auto walk = [&](auto careful) {
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt) dk[mt] = dv[mt] = f32x16{};
+    Stage ahead;
+    look(0);
+    ids(ahead, 0);
+    __syncthreads();
+    fetch(ahead, 0);
+    for (int r0 = 0; r0 < rows; r0 += NR) stage(ahead, r0, careful);
+  };
+  walk(std::false_type{});
+  // An infinite or NaN value of Q or dO spoils the keys that must not see it: the rows once
+  // more with such values as 0 in these products, the rest by add_odd_rows.
+  float worst = 0.f;  // NaN where some result is not finite
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) worst = __builtin_fmaf(dk[mt][i], 0.f, __builtin_fmaf(dv[mt][i], 0.f, worst));
+  if (__syncthreads_or(worst != 0.f)) {
+    a.kvodd[(int64_t)bh * a.nblk + desc.blk] = 1;
+    walk(std::true_type{});
+  }
+  if constexpr (DS) {
+    __syncthreads();
+    put_ds((rows - 1) / NR * NR);
   }
   // the row groups of a key, through LDS (a [32 keys][D] tile of floats for each key group), then to the item
   float* out = a.kvpart + item * 2 * KT * p.D;
@@ -676,7 +750,9 @@ __device__ __forceinline__ void add_odd_keys(const SArgs& a, f32x4& o, float lse
   };
   float qx[4];
   load(a.q, b * p.q_stride[0] + q * p.q_stride[1] + h * p.q_stride[2], qx);
+  const auto nan = [](const auto& x) { return x[0] != x[0] && x[1] != x[1] && x[2] != x[2] && x[3] != x[3]; };
   for (int64_t k = k0; k < k1; ++k) {
+    if (!group_any(!nan(o), lpr)) return;  // all NaN already
     float kx[4], vx[4];
     load(a.k, b * p.k_stride[0] + k * p.k_stride[1] + hk * p.k_stride[2], kx);
     load(a.v, b * p.v_stride[0] + k * p.v_stride[1] + hk * p.v_stride[2], vx);
@@ -706,6 +782,7 @@ __device__ __forceinline__ void add_odd_rows(const SArgs& a, float (&o)[4], int 
   const int64_t ka = b * p.k_stride[0] + key * p.k_stride[1] + hk * p.k_stride[2];
   const int64_t va = b * p.v_stride[0] + key * p.v_stride[1] + hk * p.v_stride[2];
   for (int r = 0; r < (off[1] - off[0]) * a.G; ++r) {
+    if (o[0] != o[0] && o[1] != o[1] && o[2] != o[2] && o[3] != o[3]) return;  // all NaN already
     const RowId id = row_id(a, list, r);
     if (key >= key_limit(p, b, id.q, held, first_pos(p, b))) continue;
     const int h = hk * a.G + id.g;
@@ -861,6 +938,334 @@ void join_keys(SArgs a, int KT) {
   }
   const int64_t* st = w ? p.dv_stride : p.dk_stride;
   store_v<Tag, 4>(w ? a.dv : a.dk, b * st[0] + kk * st[1] + hk * st[2] + col, o);
+}
+
+// ---- by tiles of queries --------------------------------------------------------------
+
+// Forward without partial rows: a wave holds 32 rows (32 / G neighbouring queries of a
+// key head with all their heads), a workgroup four such; it walks the blocks that any of its
+// queries selected, each row masked to its own.  The union grows with the queries of a tile,
+// but no faster than their selections together, and each block costs products (and one read
+// of K and V from the cache) where the form by blocks costs 8 D bytes of memory a row: below
+// (sel_plan).  K and V of the next tile are loaded while this tile's products run.
+//
+// lane = row, as in by_block_q.  The running maximum moves only when a score passes it by
+// 2^8 (the weights are then below 2^8, in every type's range), so that the accumulators
+// are hardly ever rescaled; a negative or zero scale is folded into Q.  A row that did not
+// select a block gets weights 0 by an infinite subtrahend; where infinite or NaN values make
+// that NaN, or spoil a product (0 times them), the result is not finite, and the workgroup
+// walks its blocks once more with every element masked and such values as 0 (add_odd_keys
+// then gives them to the rows that see them).
+//
+// GRAD: dQ = scale dS K the same way, from the dS that the dK/dV kernel has left in memory:
+// 2 bytes a pair, where a partial row of dQ takes 8 D for each row and block.
+//
+// Per wave and tile of 64 keys at D = 128: 1024 (dQ: 512) cycles of matrix products, 1280 of
+// LDS traffic a workgroup, some 850 of vector instructions (32 exponentials of 16 cycles).
+constexpr int kSpan = 512;  // blocks whose selections lie in LDS at a time
+template <class Tag, int D, bool GRAD>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(SOp<Tag>::ES == 2 ? 2 : 1)))
+void by_tile(SArgs a, int hgroups, int tiles_q) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  constexpr int NBUF = SOp<Tag>::ES == 2 ? 2 : 1;  // K and V tiles in LDS
+  __shared__ __align__(16) char lds[NBUF][(GRAD ? 1 : 2) * kKT * T::RB];
+  __shared__ uint32_t s_sel[kSpan][4];  // block, wave: the wave's queries that selected it
+  constexpr int kPos = 8192;
+  __shared__ int s_pos[GRAD ? kPos : 1];  // GRAD: block, query: where the query's dS of the block lies
+  __shared__ int s_list[kSpan], s_n, s_odd[2];
+  const mattn_selected& p = a.p;
+  int x = blockIdx.x;
+  const int bh = x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
+  x /= a.bh_n;
+  const int h0 = 32 * (x % hgroups), G = min(a.G - h0, 32), R = 32 / min(a.G, 32);  // heads, queries of a wave
+  const int q0 = (tiles_q - 1 - x / hgroups) * 4 * R;                              // late queries see most: first
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+  const int held = keys_held(p, b);
+  const int64_t start = first_pos(p, b);
+  const int qi = l32 / G, q = q0 + wave * R + qi, h = hk * a.G + h0 + l32 % G;
+  const bool live = qi < R && q < p.Lq;
+  const int qc = live ? q : p.Lq - 1;
+  const int64_t row = ((int64_t)bh * p.Lq + qc) * a.G + h0 + l32 % G;
+  const int lim = live ? key_limit(p, b, qc, held, start) : 0;
+  const bool zero = p.scale == 0.f;
+  const float sl = zero ? 1.f : fabsf(a.scale_log2);
+  typename O::Frag qf[GRAD ? 1 : D / 16];
+  if constexpr (!GRAD) {
+    load_rows<Tag, D>(qf, a.q, b * p.q_stride[0] + qc * p.q_stride[1] + h * p.q_stride[2], hi, p.D);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) qf[c] = O::sign(qf[c], p.scale < 0.f, zero);
+  }
+  float lse = GRAD ? a.lse[row] : 0.f;
+  const char* kb = (const char*)a.k + O::ES * (b * p.k_stride[0] + hk * p.k_stride[2]);
+  const char* vb = (const char*)a.v + O::ES * (b * p.v_stride[0] + hk * p.v_stride[2]);
+  // K and V of a tile, as buffers that end behind its last key: this thread's chunks lie at
+  // fixed offsets (past the end where the head is narrower than D), what is past the end is 0
+  constexpr int EC = 16 / O::ES, N = kKT * T::CPR / 256, RPI = 256 / T::CPR;
+  const int my_r = threadIdx.x / T::CPR, my_c = threadIdx.x % T::CPR;
+  const bool in_d = my_c * EC < p.D;
+  const int ksb = (int)p.k_stride[1] * O::ES, vsb = (int)p.v_stride[1] * O::ES;  // bytes of a row
+  const uint32_t k_at = in_d ? my_r * ksb + 16 * my_c : 0x80000000u, v_at = in_d ? my_r * vsb + 16 * my_c : 0x80000000u;
+  u32x4 xk[N], xv[GRAD ? 1 : N];
+  typename O::Frag xs[GRAD ? kKT / 16 : 1], cs[GRAD ? kKT / 16 : 1];  // GRAD: dS of the tile in flight, of this one
+  int64_t key0 = 0;  // first key of the tile in flight, and its keys
+  int key_n = 0;
+  int ds_at = -1, ds_key = 0;
+  const auto fetch = [&]() {
+    const auto kr = make_rsrc(kb + key0 * ksb, (uint32_t)((key_n - 1) * ksb + p.D * O::ES));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      xk[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)k_at, i * RPI * ksb, 0));
+    if constexpr (!GRAD) {
+      const auto vr = make_rsrc(vb + key0 * vsb, (uint32_t)((key_n - 1) * vsb + p.D * O::ES));
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        xv[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)v_at, i * RPI * vsb, 0));
+    } else {
+      const char* d = (const char*)a.ds + O::ES * ((((int64_t)bh * p.Lq * p.count + ds_at) * a.G + h0 + l32 % G) * p.block_size + ds_key);
+#pragma unroll
+      for (int i = 0; i < kKT / 16; ++i)
+        xs[i] = ds_at >= 0 && ds_key + 16 * i < p.block_size ? O::load(d + O::ES * (16 * i + 8 * hi)) : O::zero();
+    }
+  };
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  const int last = key_limit(p, b, min(q0 + 4 * R, p.Lq) - 1, held, start);
+  const int blocks = (last + p.block_size - 1) / p.block_size;
+  f32x16 acc[D / 32];
+  float m, sum;
+  int seq = 0;
+  bool careful = false, spoilt = false;  // spoilt: some tile held an infinite or NaN value
+  for (;; careful = true) {
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
+  m = NEG_INF, sum = 0.f;
+  const int full = GRAD ? min(kSpan, kPos / (4 * R)) : kSpan;
+  for (int lo = 0; lo < blocks; lo += full) {
+    const int span = min(full, blocks - lo);
+    __syncthreads();
+    for (int i = threadIdx.x; i < span * 4; i += 256) (&s_sel[0][0])[i] = 0u;
+    if constexpr (GRAD)
+      for (int i = threadIdx.x; i < span * 4 * R; i += 256) s_pos[i] = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4 * R * p.count; i += 256) {
+      const int t = i / p.count, qq = q0 + t;
+      if (qq >= p.Lq) break;
+      const int c = i % p.count, j = p.blocks[(((int64_t)b * p.Lq + qq) * p.Hkv + hk) * p.count + c] - lo;
+      if (j >= 0 && j < span && (int64_t)(j + lo) * p.block_size < key_limit(p, b, qq, held, start)) {
+        if constexpr (GRAD) {  // (of a repeated block the slot that counts)
+          if (!((a.ok[((int64_t)bh * p.Lq + qq) * a.words + (c >> 5)] >> (c & 31)) & 1u)) continue;
+          s_pos[j * 4 * R + t] = a.pos[((int64_t)bh * p.Lq + qq) * p.count + c];
+        }
+        atomicOr(&s_sel[j][t / R], 1u << (t % R));
+      }
+    }
+    __syncthreads();
+    if (wave == 0) {
+      int n = 0;
+      for (int j = 0; j < span; j += 64) {
+        const bool any = j + lane < span && (s_sel[j + lane][0] | s_sel[j + lane][1] | s_sel[j + lane][2] | s_sel[j + lane][3]);
+        const uint64_t bm = __ballot(any);
+        if (any) s_list[n + __builtin_popcountll(bm & ((1ull << lane) - 1))] = j + lane;
+        n += __builtin_popcountll(bm);
+      }
+      if (lane == 0) s_n = n;
+    }
+    __syncthreads();
+    const int n = __builtin_amdgcn_readfirstlane(s_n);
+    if (n == 0) continue;
+    int e = 0, t = 0;  // tile in flight: entry, tile of its block
+    bool further = false;  // the block has a tile behind it
+    uint32_t bits = 0u;    // the wave's queries that selected the block
+    const auto place = [&]() {
+      const int j = __builtin_amdgcn_readfirstlane(s_list[e]);
+      bits = __builtin_amdgcn_readfirstlane(s_sel[j][wave]);
+      const int64_t k0 = (int64_t)(lo + j) * p.block_size;
+      const int inside = (int)min((int64_t)p.block_size, held - k0);
+      key0 = k0 + t * kKT;
+      key_n = min(inside - t * kKT, kKT);
+      further = t * kKT + kKT < inside;
+      if constexpr (GRAD) {
+        ds_at = live ? s_pos[j * 4 * R + wave * R + qi] : -1;
+        ds_key = t * kKT;
+      }
+    };
+    const auto put = [&](char* kt) {  // the tile in flight to LDS
+      ++seq;
+      char* vt = kt + kKT * T::RB;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = i * RPI + my_r;
+        u32x4 last = GRAD ? xk[i] : xv[GRAD ? 0 : i];
+        if (careful && O::odd(last)) {
+          s_odd[seq & 1] = seq;  // (the other place may still be read for the tile before)
+          last = O::finite16(last);
+        }
+        if constexpr (!GRAD) *(u32x4*)(kt + T::at(r, my_c)) = xk[i];
+        *(u32x4*)((GRAD ? kt : vt) + T::at(r, my_c)) = last;
+      }
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int i = 0; i < kKT / 16; ++i) cs[i] = xs[i];
+      }
+    };
+    place();
+    fetch();
+    put(lds[0]);
+    barrier_lds();
+    int buf = 0;
+    while (e < n) {
+      const char *kt = lds[buf], *vt = kt + kKT * T::RB;
+      const int see = live && ((bits >> qi) & 1u) ? (int)min((int64_t)key_n, lim - key0) : 0;
+      spoilt = spoilt || (careful && s_odd[seq & 1] == seq);
+      if (further) {
+        ++t;
+      } else {
+        ++e;
+        t = 0;
+      }
+      if (e < n) {
+        place();
+        fetch();
+      }
+      if (__any(see > 0)) {
+        const bool slow = !GRAD && (careful || __any(see > 0 && see < kKT));  // some row sees a part of the tile
+        const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int u, float(&s)[16]) {
+          f32x16 r16 = f32x16{};
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(tile, 32 * u + l32, 2 * c + hi), f[c], r16);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = r16[i];
+        };
+        const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = s[8 * j + i];
+            f[j] = O::pack(y);
+          }
+        };
+        if constexpr (!GRAD) {
+          float s[2][16];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) scores(kt, qf, u, s[u]);
+          if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 6, 1>();
+          if (slow) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t vis = below(see - 32 * u, hi);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[u][i] = mask_neg_inf(s[u][i], seen_bit(vis, i));
+            }
+          }
+          float top = NEG_INF;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[u][i], s[u][i + 1]), top);
+          top = see > 0 ? wave_max32(top) : NEG_INF;  // (both halves of a row have one `see`)
+          if (__any((top - m) * sl > 8.f)) {          // (the first scores of a row: m is -inf)
+            const float to = fmaxf(m, top), keep = to == NEG_INF ? 1.f : fast_exp2((m - to) * sl);
+            m = to;
+            sum *= keep;
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] *= keep;
+          }
+          const float ref = see > 0 ? (m == NEG_INF ? 0.f : m * sl) : -NEG_INF;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = fast_exp2(__builtin_fmaf(s[u][i], sl, -ref));
+            typename O::Frag f[2];
+            operands(s[u], f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              sum = O::total(f[j], sum);
+#pragma unroll
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * u + j, mt, lane), f[j], acc[mt]);
+            }
+          }
+          if constexpr (O::ES == 2) reads_ahead<4 * D / 32, 6, 2>();
+        } else {
+#pragma unroll
+          for (int i = 0; i < kKT / 16; ++i)
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32n(kt, i, mt, lane), cs[i], acc[mt]);
+          if constexpr (O::ES == 2) reads_ahead<kKT / 16 * D / 32, 6, 2>();
+        }
+      }
+      if constexpr (NBUF == 2) buf ^= 1;
+      else barrier_lds();  // all are done with the one buffer
+      if (e < n) put(lds[buf]);
+      barrier_lds();
+    }
+  }
+  if (careful) break;
+  float worst = 0.f;  // NaN where some result is not finite
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) worst = __builtin_fmaf(acc[mt][i], 0.f, worst);
+  if (!__syncthreads_or(live && worst != 0.f)) break;
+  }
+
+  const int64_t* os = GRAD ? p.dq_stride : p.o_stride;
+  char* out = (char*)(GRAD ? a.dq : a.o);
+  float r = p.scale;
+  if constexpr (!GRAD) {
+    sum = wave_sum32(sum);
+    r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    lse = sum > 0.f || sum != sum ? __builtin_fmaf(m, sl, __log2f(sum)) : NEG_INF;
+  }
+  if (live) {
+    const int64_t at = b * os[0] + qc * os[1] + h * os[2];
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 32 * mt + 8 * j + 4 * hi;
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = acc[mt][4 * j + i] * r;
+        if (c < p.D) {
+          store_v<Tag, 4>(out, at + c, y);
+          if (!GRAD && a.o32) *(f32x4*)(a.o32 + row * p.D + c) = f32x4{y[0], y[1], y[2], y[3]};
+        }
+      }
+    if (!GRAD && a.lse && hi == 0) a.lse[row] = lse;
+  }
+  if (!spoilt) return;
+  // what the infinite and NaN values give to the rows that see them
+  float* s_lse = (float*)lds[0];
+  __syncthreads();
+  if (live && hi == 0) s_lse[32 * wave + l32] = lse;
+  __syncthreads();
+  int lpr = 2;
+  while (4 * lpr < p.D) lpr *= 2;
+  const int col = 4 * (threadIdx.x & (lpr - 1));
+  for (int y = threadIdx.x / lpr; y < 128; y += 256 / lpr) {
+    const int wi = y >> 5, ri = y & 31, yq = q0 + wi * R + ri / G, yg = h0 + ri % G;
+    if (ri / G >= R || yq >= p.Lq) continue;
+    const int64_t yrow = ((int64_t)bh * p.Lq + yq) * a.G + yg, at = b * os[0] + yq * os[1] + (int64_t)(hk * a.G + yg) * os[2] + col;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < p.count; ++c) {
+      const int j = p.blocks[(((int64_t)b * p.Lq + yq) * p.Hkv + hk) * p.count + c];
+      if (j >= 0 && j < a.nblk) add_odd_keys<Tag, GRAD>(a, o, s_lse[y], yrow, b, hk, hk * a.G + yg, yq, j, col, lpr);
+    }
+    if (col < p.D && (o[0] != 0.f || o[1] != 0.f || o[2] != 0.f || o[3] != 0.f)) {
+      float z[4];
+      load_v<Tag, 4>(out, at, z);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] += o[i];
+      store_v<Tag, 4>(out, at, z);
+      if (!GRAD && a.o32) {
+        f32x4 w = *(const f32x4*)(a.o32 + yrow * p.D + col);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += o[i];
+        *(f32x4*)(a.o32 + yrow * p.D + col) = w;
+      }
+    }
+  }
 }
 
 // ---- by queries -----------------------------------------------------------------------
@@ -1093,7 +1498,7 @@ int sel_check(const mattn_selected* p) {
 }
 
 struct SPlan {
-  bool by_query;
+  bool by_query, tile_fwd, tile_bwd;
   int splits, hgroups;
 };
 
@@ -1104,6 +1509,24 @@ SPlan sel_plan(const mattn_selected* p) {
   s.hgroups = (int)cdiv(G, 16);
   const int64_t wgs = bh * p->Lq * s.hgroups, tiles = cdiv((int64_t)p->count * p->block_size, 32);
   s.by_query = p->Lq <= 16;
+  // By tiles or by blocks.  A wave's tile holds R queries; where their selections are
+  // independent its union has U = v (1 - (1 - n / v)^R) of the v blocks they see on average
+  // (neighbouring queries share more, which favours tiles).  Measured at D = 128 in 16 bits,
+  // ns: by tiles 1.4 a wave and 64 keys (dQ 1.0, and 0.03 a row for writing dS), by blocks
+  // 0.24 + 0.08 a row and 64 keys (dQ 0.26 + 0.11), 32 rows a wave: at 64 keys a block tiles
+  // up to U = 7.3 n (dQ 11 n), at 512 keys 2.5 n (3.6 n).  [1, 8192, 32/8, 128], 16 blocks of
+  // 64: forward 0.58 ms against 1.36, backward 1.1 against 2.2; [1, 65536, 2, 128]: 2.0 against
+  // 0.81 and 1.9 against 1.3.  Float32 products take eight times as long: forward up to 1.9 n
+  // at 64 keys, dQ by blocks.
+  const double R = G < 32 ? 32 / G : 1, T = (double)cdiv(p->block_size, 64), n = p->count;
+  const double v = fmax(n, (double)cdiv(p->Lk, p->block_size) * (p->causal && !p->starts ? 0.5 : 1.0));
+  const double U = v * (1.0 - pow(1.0 - n / v, R));
+  const int es = p->dtype == MATTN_F32 ? 4 : 2;
+  // (a tile's keys are read through buffers with 32-bit offsets)
+  const bool fits = p->k_stride[1] < (1 << 30) / (64 * es) && p->v_stride[1] < (1 << 30) / (64 * es);
+  const bool f32 = p->dtype == MATTN_F32;
+  s.tile_fwd = !s.by_query && fits && (f32 ? U < 1.9 * n && T == 1 : U * T < n * (5.4 + 1.9 * T));
+  s.tile_bwd = fits && !f32 && U * T < n * (8.3 + 2.6 * T);
   s.splits = 1;
   while (s.splits < 32 && wgs * s.splits < 512 && tiles / (2 * s.splits) >= 4) s.splits *= 2;
   return s;
@@ -1111,10 +1534,10 @@ SPlan sel_plan(const mattn_selected* p) {
 
 struct SLayout {
   // lists: kept for the backward
-  size_t ok, off, kvoff, ent, tile, kvtile, lists;
+  size_t ok, off, kvoff, ent, pos, tile, kvtile, lists;
   // workspace
   size_t cnt, odd, part, plse, fwd;                   // forward
-  size_t delta, dqpart, kvpart, bodd, kvodd, bwd;  // backward
+  size_t delta, dqpart, ds, kvpart, bodd, kvodd, bwd;  // backward
   int words, chunks, nblk, max_tiles, max_kv, subs;
 };
 
@@ -1139,12 +1562,13 @@ SLayout sel_layout(const mattn_selected* p) {
   l.off = take(bh * (l.nblk + 1) * 4);
   l.kvoff = take(bh * (l.nblk + 1) * 4);
   l.ent = take(bh * most * 4);
+  l.pos = take(bh * most * 4);
   l.tile = take(bh * l.max_tiles * sizeof(Desc));
   l.kvtile = take(bh * l.max_kv * sizeof(Desc));
   l.lists = x;
   x = 0;
   const SPlan s = sel_plan(p);
-  const int64_t slots = s.by_query ? (s.splits > 1 ? s.splits : 0) : p->count;
+  const int64_t slots = s.by_query ? (s.splits > 1 ? s.splits : 0) : s.tile_fwd ? 0 : p->count;
   l.cnt = take(bh * l.nblk * l.chunks * 4);
   l.odd = take(bh * l.nblk * 4);
   l.part = take(rows * slots * p->D * 4);
@@ -1152,7 +1576,8 @@ SLayout sel_layout(const mattn_selected* p) {
   l.fwd = x;
   x = 0;
   l.delta = take(rows * 4);
-  l.dqpart = take(rows * p->count * p->D * 4);
+  if (s.tile_bwd) l.ds = take(rows * p->count * p->block_size * (p->dtype == MATTN_F32 ? 4 : 2));
+  else l.dqpart = take(rows * p->count * p->D * 4);
   l.kvpart = take(bh * l.max_kv * 2 * key_tile(p) * p->D * 4);
   l.bodd = take(bh * l.nblk * 4);
   l.kvodd = take(bh * l.nblk * 4);
@@ -1178,6 +1603,7 @@ SArgs sel_args(const mattn_selected* p, const SLayout& l, void* lists) {
     a.off = (int*)(c + l.off);
     a.kvoff = (int*)(c + l.kvoff);
     a.ent = (int*)(c + l.ent);
+    a.pos = (int*)(c + l.pos);
     a.tile = (Desc*)(c + l.tile);
     a.kvtile = (Desc*)(c + l.kvtile);
   }
@@ -1232,7 +1658,7 @@ extern "C" size_t mattn_selected_lists_bytes(const mattn_selected* p) { return s
 extern "C" size_t mattn_selected_fwd_workspace_bytes(const mattn_selected* p) {
   if (sel_check(p)) return 0;
   const SLayout l = sel_layout(p);
-  return sel_plan(p).by_query ? l.fwd : l.fwd + l.lists;
+  return l.fwd + (sel_plan(p).by_query || sel_plan(p).tile_fwd ? 0 : l.lists);
 }
 
 extern "C" size_t mattn_selected_bwd_workspace_bytes(const mattn_selected* p) { return sel_check(p) ? 0 : sel_layout(p).bwd; }
@@ -1262,21 +1688,25 @@ extern "C" int mattn_selected_fwd(const mattn_selected* p, const void* q, const 
   a.odd = (int*)(ws + l.odd);
   a.part = (float*)(ws + l.part);
   a.plse = (float*)(ws + l.plse);
-  if (grads || !s.by_query) make_lists(a, st);
+  if (grads || !(s.by_query || s.tile_fwd)) make_lists(a, st);
   const int ll = lanes_log2(p->D);
   const int64_t rows = (int64_t)a.bh_n * p->Lq * a.G;
   const dim3 join((uint32_t)cdiv(rows << ll, 256));
+  const int hg32 = (a.G + 31) / 32, tiles_q = (int)cdiv(p->Lq, 4 * (32 / (a.G < 32 ? a.G : 32)));
+  const dim3 tiles((uint32_t)((int64_t)a.bh_n * hg32 * tiles_q));
   with_type(p->dtype, [&](auto tag) {
     using Tag = decltype(tag);
     with_dim(p->D, [&](auto dim) {
       constexpr int D = decltype(dim)::value;
       if (s.by_query)
         hipLaunchKernelGGL((by_query<Tag, D>), dim3((uint32_t)(a.bh_n * p->Lq * s.hgroups * s.splits)), dim3(256), 0, st, a, s.splits, s.hgroups);
+      else if (s.tile_fwd)
+        hipLaunchKernelGGL((by_tile<Tag, D, false>), tiles, dim3(256), 0, st, a, hg32, tiles_q);
       else
         hipLaunchKernelGGL((by_block_q<Tag, D, false>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
     });
-    if (!s.by_query) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, p->count, false);
-    else if (s.splits > 1) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, s.splits, true);
+    if (!s.by_query && !s.tile_fwd) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, p->count, false);
+    else if (s.by_query && s.splits > 1) hipLaunchKernelGGL((join_rows<Tag, false>), join, dim3(256), 0, st, a, ll, s.splits, true);
   });
   return hipGetLastError() == hipSuccess ? MATTN_OK : MATTN_ERR_LAUNCH;
 }
@@ -1303,7 +1733,9 @@ extern "C" int mattn_selected_bwd(const mattn_selected* p, const void* q, const 
   a.dv = dv;
   a.delta = (float*)(ws + l.delta);
   a.part = (float*)(ws + l.dqpart);
+  const SPlan s = sel_plan(p);
   a.kvpart = (float*)(ws + l.kvpart);
+  a.ds = s.tile_bwd ? ws + l.ds : nullptr;
   a.odd = (int*)(ws + l.bodd);
   a.kvodd = (int*)(ws + l.kvodd);
   const int ll = lanes_log2(p->D);
@@ -1311,16 +1743,30 @@ extern "C" int mattn_selected_bwd(const mattn_selected* p, const void* q, const 
   const dim3 join((uint32_t)cdiv(rows << ll, 256));
   const int KT = key_tile(p);
   const dim3 keys((uint32_t)cdiv((int64_t)p->Lk * (p->D / 4), 256), 2 * a.bh_n);
+  const int hg32 = (a.G + 31) / 32, tiles_q = (int)cdiv(p->Lq, 4 * (32 / (a.G < 32 ? a.G : 32)));
+  const dim3 tiles((uint32_t)((int64_t)a.bh_n * hg32 * tiles_q));
   with_type(p->dtype, [&](auto tag) {
     using Tag = decltype(tag);
     hipLaunchKernelGGL((row_delta<Tag>), join, dim3(256), 0, st, a, ll);
     with_dim(p->D, [&](auto dim) {
       constexpr int D = decltype(dim)::value;
-      hipLaunchKernelGGL((by_block_q<Tag, D, true>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
-      if (KT == 128) hipLaunchKernelGGL((by_block_kv<Tag, D, 128>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((by_block_kv<Tag, D, 64>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(256), 0, st, a);
+      if (!s.tile_bwd) hipLaunchKernelGGL((by_block_q<Tag, D, true>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
+      const auto kv = [&](auto kt, auto ds) {
+        hipLaunchKernelGGL((by_block_kv<Tag, D, decltype(kt)::value, decltype(ds)::value>), dim3((uint32_t)(a.bh_n * l.max_kv)),
+                           dim3(256), 0, st, a);
+      };
+      using K64 = std::integral_constant<int, 64>;
+      using K128 = std::integral_constant<int, 128>;
+      if constexpr (!std::is_same_v<Tag, float>) {
+        if (s.tile_bwd) {
+          KT == 128 ? kv(K128{}, std::true_type{}) : kv(K64{}, std::true_type{});
+          hipLaunchKernelGGL((by_tile<Tag, D, true>), tiles, dim3(256), 0, st, a, hg32, tiles_q);
+          return;
+        }
+      }
+      KT == 128 ? kv(K128{}, std::false_type{}) : kv(K64{}, std::false_type{});
     });
-    hipLaunchKernelGGL((join_rows<Tag, true>), join, dim3(256), 0, st, a, ll, p->count, false);
+    if (!s.tile_bwd) hipLaunchKernelGGL((join_rows<Tag, true>), join, dim3(256), 0, st, a, ll, p->count, false);
     hipLaunchKernelGGL((join_keys<Tag>), keys, dim3(256), 0, st, a, KT);
   });
   return hipGetLastError() == hipSuccess ? MATTN_OK : MATTN_ERR_LAUNCH;

@@ -36,12 +36,30 @@ struct SOp {  // 16-bit
   }
   static __device__ __forceinline__ Frag zero() { return Frag{0u, 0u, 0u, 0u}; }
   static __device__ __forceinline__ Frag load(const void* p) { return *(const Frag*)p; }
-  static __device__ __forceinline__ bool odd(const u32x4& x) {  // a value that is infinite or NaN among 8
-    constexpr uint32_t E = std::is_same_v<Tag, bf16_tag> ? 0x7f80u : 0x7c00u;
-    bool any = false;
+  // a value that is infinite or NaN among 8: its exponent plus one unit carries into the sign's place
+  static __device__ __forceinline__ bool odd(const u32x4& x) {
+    constexpr uint32_t E = std::is_same_v<Tag, bf16_tag> ? 0x7f807f80u : 0x7c007c00u, U = E & -E & 0xffffu;
+    uint32_t any = 0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) any = any || (x[i] & E) == E || (x[i] & (E << 16)) == (E << 16);
-    return any;
+    for (int i = 0; i < 4; ++i) any |= (x[i] & E) + (U << 16 | U);
+    return any & 0x80008000u;
+  }
+  // c + the sum of an operand's values
+  static __device__ __forceinline__ float total(const Frag& x, float c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = x[i];  // (a bit cast of the element itself reads element 0)
+      if constexpr (std::is_same_v<Tag, bf16_tag>)
+        c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
+      else
+        c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
+    }
+    return c;
+  }
+  static __device__ __forceinline__ Frag sign(Frag x, bool neg, bool zero) {  // -x, 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = zero ? 0u : neg ? x[i] ^ 0x80008000u : x[i];
+    return x;
   }
   static __device__ __forceinline__ Frag finite(Frag x) { return finite16(x); }
   static __device__ __forceinline__ u32x4 finite16(u32x4 x) {  // such values as 0
@@ -81,6 +99,19 @@ struct SOp<float> {
     for (int i = 0; i < 4; ++i) any = any || (x[i] & 0x7f800000u) == 0x7f800000u;
     return any;
   }
+  static __device__ __forceinline__ float total(const Frag& x, float c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c += x.a[i] + x.b[i];
+    return c;
+  }
+  static __device__ __forceinline__ Frag sign(Frag x, bool neg, bool zero) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x.a[i] = zero ? 0.f : neg ? -x.a[i] : x.a[i];
+      x.b[i] = zero ? 0.f : neg ? -x.b[i] : x.b[i];
+    }
+    return x;
+  }
   static __device__ __forceinline__ u32x4 finite16(u32x4 x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = (x[i] & 0x7f800000u) == 0x7f800000u ? 0u : x[i];
@@ -95,6 +126,20 @@ struct SOp<float> {
     return x;
   }
 };
+
+// Order of a stretch of code with N products whose operands take R LDS reads each: the
+// reads of AHEAD products first, then a product and the reads of a later one in turn.
+// (Left to itself the compiler issues each read right before its product and waits.)
+template <int N, int AHEAD, int R>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
 
 // A tile of rows of D elements in LDS, packed, 16-byte chunk c of row r at c ^ f(r): row
 // reads (16 rows at one chunk) and transposed reads (4 rows at 4 chunks) then touch all
@@ -138,6 +183,24 @@ struct STile {
       for (int e = 0; e < 4; ++e) {
         o.a[e] = elem(t, r + e, c);
         o.b[e] = elem(t, r + 8 + e, c);
+      }
+      return o;
+    }
+  }
+  // The same in the order of an operand read along its rows (slot e: row 16 j + 8 hi + e)
+  static __device__ __forceinline__ typename O::Frag tr32n(const char* t, int j, int mt, int lane) {
+    const int hi = lane >> 5, r = 16 * j + 8 * hi;
+    if constexpr (O::ES == 2) {
+      const int c0 = 32 * mt + 16 * ((lane >> 4) & 1);
+      const u32x2 x = tr4(t, r, c0, lane), y = tr4(t, r + 4, c0, lane);
+      return u32x4{x[0], x[1], y[0], y[1]};
+    } else {
+      const int c = 32 * mt + (lane & 31);
+      F8 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o.a[e] = elem(t, r + e, c);
+        o.b[e] = elem(t, r + 4 + e, c);
       }
       return o;
     }

@@ -171,6 +171,11 @@ SHAPES = [
     (1, 1, 1, 1, 1, 8, 16, 1), (2, 40, 40, 4, 2, 64, 16, 3), (1, 300, 300, 8, 2, 64, 64, 3), (2, 129, 260, 6, 6, 128, 32, 5),
     (1, 700, 700, 4, 1, 128, 64, 6), (1, 200, 500, 3, 1, 80, 128, 3), (1, 150, 600, 2, 2, 64, 256, 2),
     (2, 60, 100, 40, 2, 64, 16, 4), (1, 400, 400, 2, 1, 40, 48, 40), (1, 90, 333, 4, 2, 20, 80, 3), (1, 2300, 260, 2, 1, 64, 64, 2),
+    # few of many blocks for many queries of one head: by blocks, not by tiles of queries
+    (1, 700, 700, 2, 2, 64, 16, 1), (2, 400, 900, 1, 1, 128, 16, 2), (1, 500, 2000, 2, 1, 96, 16, 1), (1, 300, 4096, 1, 1, 128, 256, 1),
+    (1, 300, 2048, 2, 2, 64, 128, 1),
+    # more blocks than a workgroup holds the selections of at a time
+    (1, 130, 9000, 2, 2, 64, 16, 30), (1, 40, 20000, 1, 1, 64, 16, 200),
 ]
 
 
@@ -225,15 +230,20 @@ def test_served_tokens(N, Hq, bs, count, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
-@pytest.mark.parametrize("bs", [32, 128])
-def test_odd_values_stay_with_the_queries_that_see_them(dtype, bs):
-    """NaN and infinities in a token reach no query before it, in any output."""
+@pytest.mark.parametrize("bs,N", [(32, 200), (128, 200), (16, 1200)])
+def test_odd_values_stay_with_the_queries_that_see_them(dtype, bs, N):
+    """NaN and infinities in a token reach no query before it, in any output.  (1200
+    queries with their own block alone run by blocks.)"""
     import jaxmodules_amd as jm
 
     gen = _gen(8)
-    N = 200
-    q, k, v, do = (_normal(gen, 1, N, h, 64, dtype=dtype) for h in (4, 2, 2, 4))
-    blocks = torch.arange(-(-N // bs), device="cuda", dtype=torch.int32).expand(1, N, 2, -1).contiguous()
+    own = N > 1000
+    hq = 2 if own else 4
+    q, k, v, do = (_normal(gen, 1, N, h, 64, dtype=dtype) for h in (hq, 2, 2, hq))
+    if own:
+        blocks = (torch.arange(N, device="cuda", dtype=torch.int32) // bs)[None, :, None, None].expand(1, N, 2, 1).contiguous()
+    else:
+        blocks = torch.arange(-(-N // bs), device="cuda", dtype=torch.int32).expand(1, N, 2, -1).contiguous()
 
     def grads(q, k, v, do):
         x = [t.clone().requires_grad_() for t in (q, k, v)]
