@@ -89,8 +89,8 @@ def test_c_entries_refuse():
     bwd = lambda n, dk=a: lib.mattn_selected_bwd(_struct(), a, a, a, a, a, a, a, a, n, a, dk, a, None)  # noqa: E731
     assert n > 0 and bwd(n - 1) == -11 and bwd(n, dk=None) == -1 and bwd(n, dk=a + 4) == -5
     s = _lib.MattnSelect(B=1, L=1, nblk=4, Hq=2, Hkv=1, D=64, dtype=0, block_size=16, count=2, first=1, last=1, q=a, means=a, blocks=a)
-    assert lib.mattn_select_workspace_bytes(ctypes.byref(s)) == 32
-    assert lib.mattn_select_blocks(ctypes.byref(s), None, 32, None) == -1 and lib.mattn_select_blocks(ctypes.byref(s), a, 31, None) == -11
+    n = lib.mattn_select_workspace_bytes(ctypes.byref(s))
+    assert n >= 16 and lib.mattn_select_blocks(ctypes.byref(s), None, n, None) == -1 and lib.mattn_select_blocks(ctypes.byref(s), a, n - 1, None) == -11
     for field, bad, code in (("first", 2, -2), ("D", 12, -3), ("dtype", 9, -4), ("means", None, -1), ("q", a + 2, -5), ("Hkv", 3, -2)):
         was = getattr(s, field)
         setattr(s, field, bad)
