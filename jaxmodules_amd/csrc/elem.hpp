@@ -43,6 +43,31 @@ __device__ __forceinline__ void load_v(const void* base, int64_t e, float (&o)[V
   }
 }
 
+// The same as they lie in memory, and as float.
+template <class Tag, int V>
+using Raw = std::conditional_t<V == 1, std::conditional_t<std::is_same_v<Tag, float>, float, uint16_t>, u32x4>;
+template <class Tag, int V>
+__device__ __forceinline__ Raw<Tag, V> load_raw(const void* base, int64_t e) {
+  return *(const Raw<Tag, V>*)((const char*)base + (std::is_same_v<Tag, float> ? 4 : 2) * e);
+}
+template <class Tag, int V>
+__device__ __forceinline__ void from_raw(const Raw<Tag, V>& x, float (&o)[V]) {
+  if constexpr (std::is_same_v<Tag, float>) {
+    if constexpr (V == 1) {
+      o[0] = x;
+    } else {
+      const f32x4 y = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = y[i];
+    }
+  } else if constexpr (V == 1) {
+    o[0] = Elt<Tag>::to_f32(x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = Elt<Tag>::to_f32(elt16(x, i));
+  }
+}
+
 template <class Tag, int V>
 __device__ __forceinline__ void store_v(void* base, int64_t e, const float (&o)[V]) {
   if constexpr (std::is_same_v<Tag, float>) {

@@ -112,8 +112,10 @@ class _Call:
         if not self.norm:  # (of a linear map that keeps lengths: the turn back)
             return self.forward(gs, inverse=True), None
         ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-        dw = [torch.zeros(x.shape[3], dtype=torch.float32, device=x.device) if weights_too else None for x in xs]
         live = [t for t, x in enumerate(xs) if x.numel()]
+        # (a tensor of no rows is left out of the launch, and its weight's gradient zero)
+        dw = [(torch.empty if x.numel() else torch.zeros)(x.shape[3], dtype=torch.float32, device=x.device) if weights_too else None
+              for x in xs]
         if live:
             lib = _lib.load()
             p = self.only(live).record([xs[t] for t in live], [ys[t] for t in live], [gs[t] for t in live])
@@ -151,7 +153,8 @@ class _Rotary(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *gs):
         gs = [rows(g) for g in gs]
-        xs = ctx.saved_tensors[-ctx.n:] if ctx.call.norm else gs
+        saved = ctx.saved_tensors  # (read in any case: that is where a changed one is noticed)
+        xs = saved[-ctx.n:] if ctx.call.norm else gs
         weights_too = any(ctx.needs_input_grad[2 + ctx.n:])
         dx, dw = ctx.call.backward(xs, gs, weights_too)
         dws = [None if dt is None or not weights_too else w.to(dt) for dt, w in zip(ctx.given, dw or [None] * len(ctx.given))]

@@ -197,6 +197,20 @@ def test_changed_weights_before_the_backward_are_an_error():
             o.sum().backward()
 
 
+@pytest.mark.parametrize("which", ["positions", "inv_freq"])
+def test_changed_angles_before_the_backward_are_an_error(which):
+    """Without the norm nothing else is kept for the backward, and these are."""
+    import jaxmodules_amd as jm
+
+    q = torch.randn(1, 3, 2, 64, device="cuda", requires_grad=True)
+    f, _ = _freq(32)
+    t = dict(positions=torch.arange(3, device="cuda"), inv_freq=f.clone())
+    o = jm.rotary(q, **t)
+    t[which].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+
+
 def test_gradient_against_differences():
     """(f(x + h) - f(x - h)) / 2 of the entry point itself, in float32: h^2 of the third
     derivative and u / h of the values, both below 1e-2 of the gradient's size here."""
