@@ -401,7 +401,7 @@ int mattn_block_means(const mattn_means* p, void* stream);
  * blocks below ceil(lengths[b] / block_size) (NULL: nblk) and, causal, up to its own
  * position's.  Of those the `first` first and `last` last are taken, then the best of the
  * others by the score (sum over the group's heads of q) . mean in float64, ties to the
- * lower index, NaN lowest.  D % 8 == 0, D <= 256; 16-byte aligned rows.
+ * lower index, NaN lowest.  D % 8 == 0, D <= 128; 16-byte aligned rows.
  */
 typedef struct mattn_select {
   int32_t B, L, nblk, Hq, Hkv, D;
@@ -431,7 +431,7 @@ typedef struct mattn_selected {
   int32_t B, Lq, Lk, Hq, Hkv, D;
   int32_t dtype;
   int32_t block_size, count, causal;
-  float scale;                 /* of the scores; finite */
+  float scale;                 /* of the scores; finite, times log2 e too */
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
   int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   const int32_t* blocks;

@@ -32,17 +32,18 @@ __device__ __forceinline__ int held_of(const int32_t* lengths, int b, int most) 
 // eighth key (32 chunks are 512 bytes of a row).  Bound by HBM: each key is read once.
 template <class Tag, int V>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
-void block_means(mattn_means p, int nblk) {
+void block_means(mattn_means p, int nblk, uint32_t groups) {
   __shared__ double red[8][32 * V];
   const int cc = threadIdx.x & 31, kr = threadIdx.x >> 5;
-  const int b = blockIdx.z, held = held_of(p.lengths, b, p.L);
-  int j = blockIdx.y;
+  const int b = blockIdx.y, held = held_of(p.lengths, b, p.L);
+  int j = (int)(blockIdx.x / groups);
+  const int64_t c0 = 32 * (int64_t)(blockIdx.x % groups);  // first chunk
   if (p.new_keys > 0) {  // only the blocks that hold one of the newest keys
     j += max(held - p.new_keys, 0) / p.block_size;
     if ((int64_t)j * p.block_size >= held) return;
   }
   const int cpr = p.D / V;  // chunks of a head's row
-  const int64_t c = (int64_t)blockIdx.x * 32 + cc;
+  const int64_t c = c0 + cc;
   const int h = (int)(c / cpr), col = V * (int)(c % cpr);
   const int64_t k0 = (int64_t)j * p.block_size;
   const int n = (int)min((int64_t)p.block_size, max((int64_t)held - k0, (int64_t)0));
@@ -62,7 +63,7 @@ void block_means(mattn_means p, int nblk) {
   for (int e = 0; e < V; ++e) red[kr][cc + 32 * e] = s[e];
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * V; i += 256) {
-    const int64_t ci = (int64_t)blockIdx.x * 32 + i / V;
+    const int64_t ci = c0 + i / V;
     const int hi = (int)(ci / cpr), e = i % V;
     if (hi >= p.H) continue;
     double t = 0.0;
@@ -186,9 +187,9 @@ void scores_mfma(SelArgs a, int span) {
 }
 
 // Few rows: bound by reading the means once.  16 lanes take a block's mean, 8 columns
-// each (two steps at D > 128), for all rows; the summed queries lie in LDS.
+// each, for all rows; the summed queries lie in LDS.
 constexpr int kFewRows = 8;
-constexpr int kMaxD = 256;
+constexpr int kMaxD = 128;
 template <class Tag>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
 void scores_few(SelArgs a, int per_group) {
@@ -208,12 +209,12 @@ void scores_few(SelArgs a, int per_group) {
   const float* m = p.means + b * p.m_stride[0] + hk * p.m_stride[2];
   constexpr int NB = 4;  // blocks of a group in flight
   for (int t = 0; t < per_group; t += NB) {
-    f32x4 x[NB][4];
+    f32x4 x[NB][2];
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       const int j = j0 + 16 * (t + u) + (threadIdx.x >> 4);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         const int col = 64 * c + 4 * l16;
         x[u][c] = t + u < per_group && j < most && col < p.D ? *(const f32x4*)(m + j * p.m_stride[1] + col) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
@@ -225,7 +226,7 @@ void scores_few(SelArgs a, int per_group) {
       for (int r = 0; r < rows; ++r) {
         double s = 0.0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           const int col = 64 * c + 4 * l16;
           if (col < p.D) {
 #pragma unroll
@@ -309,9 +310,9 @@ __device__ __forceinline__ void choose_exactly(const SelArgs& a, int bh, int r, 
   const mattn_select& p = a.p;
   const Row o = row_of(a, bh, r);
   const float* s = (const float*)a.s + ((int64_t)bh * a.rows + r) * p.nblk;
-  double qs[4];  // the summed query, columns lane + 64 c
+  double qs[2];  // the summed query, columns lane + 64 c
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     qs[c] = 0.0;
     const int col = lane + 64 * c, G = p.Hq / p.Hkv;
     if (col < p.D)
@@ -348,7 +349,7 @@ __device__ __forceinline__ void choose_exactly(const SelArgs& a, int bh, int r, 
         const float* row = means + (int64_t)(l + 64 * i) * p.m_stride[1];
         double x = 0.0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
           if (lane + 64 * c < p.D) x += qs[c] * (double)row[lane + 64 * c];
 #pragma unroll
         for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
@@ -359,7 +360,7 @@ __device__ __forceinline__ void choose_exactly(const SelArgs& a, int bh, int r, 
       const float* row = means + (int64_t)(mine ? lane + 64 * i : o.c0) * p.m_stride[1];
       double x = 0.0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 2; ++c)
         for (int d = 0; d < 64 && 64 * c + d < p.D; ++d) x += __shfl(qs[c], d) * (double)row[64 * c + d];
       if (mine) key[i] = order_key(x);
     }
@@ -573,8 +574,7 @@ void launch_scores(const SelArgs& a, hipStream_t st) {
     while (span > 64 && (int64_t)tiles * bh * ((p.nblk + span - 1) / span) < 1024) span /= 2;
     const dim3 grid(tiles, (p.nblk + span - 1) / span, bh);
     if (p.D <= 64) hipLaunchKernelGGL((scores_mfma<Tag, 2>), grid, dim3(256), 0, st, a, span);
-    else if (p.D <= 128) hipLaunchKernelGGL((scores_mfma<Tag, 4>), grid, dim3(256), 0, st, a, span);
-    else hipLaunchKernelGGL((scores_mfma<Tag, 8>), grid, dim3(256), 0, st, a, span);
+    else hipLaunchKernelGGL((scores_mfma<Tag, 4>), grid, dim3(256), 0, st, a, span);
     return;
   }
   // enough workgroups to fill the card, at most 16 blocks a group of 16 lanes
@@ -613,11 +613,14 @@ extern "C" int mattn_block_means(const mattn_means* p, void* stream) {
   const int nblk = (int)(((int64_t)p->L + p->block_size - 1) / p->block_size);
   const int nj = p->new_keys > 0 ? (int)((p->new_keys + (int64_t)p->block_size - 2) / p->block_size) + 1 : nblk;
   const int64_t chunks = (int64_t)p->H * p->D / (vec ? V : 1);
-  if (p->B > 65535 || nj > 65535 || nj <= 0 || (chunks + 31) / 32 >= (1ll << 31)) return MATTN_ERR_TOO_LARGE;
-  const dim3 grid((uint32_t)((chunks + 31) / 32), nj, p->B);
+  const int64_t groups = (chunks + 31) / 32;
+  if (p->B > 65535 || nj <= 0 || groups * nj >= (1ll << 31)) return MATTN_ERR_TOO_LARGE;
+  const dim3 grid((uint32_t)(groups * nj), p->B);
   const auto go = [&](auto tag) {
-    if (vec) hipLaunchKernelGGL((block_means<decltype(tag), kChunk<decltype(tag)>>), grid, dim3(256), 0, (hipStream_t)stream, *p, nblk);
-    else hipLaunchKernelGGL((block_means<decltype(tag), 1>), grid, dim3(256), 0, (hipStream_t)stream, *p, nblk);
+    if (vec) hipLaunchKernelGGL((block_means<decltype(tag), kChunk<decltype(tag)>>), grid, dim3(256), 0, (hipStream_t)stream, *p, nblk,
+                                (uint32_t)groups);
+    else hipLaunchKernelGGL((block_means<decltype(tag), 1>), grid, dim3(256), 0, (hipStream_t)stream, *p, nblk,
+                                (uint32_t)groups);
   };
   if (p->dtype == MATTN_BF16) go(bf16_tag{});
   else if (p->dtype == MATTN_F16) go(f16_tag{});

@@ -37,6 +37,7 @@ constexpr int kSlotBits = 10;   // of a list entry
 constexpr int kMaxSel = 1 << kSlotBits;  // blocks of a query
 constexpr int kRows = 512;      // rows (query, head) of a block that a forward or dQ workgroup takes
 constexpr int kRowsKV = 2048;   // rows that a dK/dV workgroup takes
+constexpr int kMaxDS = 1024;    // keys of a block whose dS is kept in memory
 
 struct Desc {
   int blk, row0;  // block (-1: idle) and first row of its list
@@ -354,105 +355,105 @@ void by_block_q(SArgs a) {
     float m, sum, exact;
     const auto walk = [&](auto careful) {
 #pragma unroll
-    for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
-    m = NEG_INF, sum = exact = 0.f;
-    for (int t = 0; t < tiles; ++t) {
-      if (tiles > 1 || (r0 == 0 && !decltype(careful)::value)) {
-        __syncthreads();
-        const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
-        const bool vo = stage_keys<Tag, D, kKT, !GRAD>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
-        if (GRAD ? ko : vo) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
-        if constexpr (GRAD) odd = __syncthreads_or(ko) || odd;
-        else __syncthreads();
-      }
-      const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
-      // S^T of 32 keys: single floats from here on (of a 16-register result changed in a branch
-      // the compiler has written back registers of another value)
-      const auto scores = [&](const char* t, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
-        f32x16 r16 = f32x16{};
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(t, 32 * x + l32, 2 * c + hi), f[c], r16);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = r16[i];
-      };
-      const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = s[8 * j + i];
-          f[j] = O::pack(e);
+      for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
+      m = NEG_INF, sum = exact = 0.f;
+      for (int t = 0; t < tiles; ++t) {
+        if (tiles > 1 || (r0 == 0 && !decltype(careful)::value)) {
+          __syncthreads();
+          const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+          const bool vo = stage_keys<Tag, D, kKT, !GRAD>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+          if (GRAD ? ko : vo) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
+          if constexpr (GRAD) odd = __syncthreads_or(ko) || odd;
+          else __syncthreads();
         }
-      };
-      if constexpr (!GRAD) {
-        float s[2][16], top = NEG_INF;
+        const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
+        // S^T of 32 keys: single floats from here on (of a 16-register result changed in a branch
+        // the compiler has written back registers of another value)
+        const auto scores = [&](const char* t, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
+          f32x16 r16 = f32x16{};
 #pragma unroll
-        for (int x = 0; x < 2; ++x) scores(kt, now.q, x, s[x]);
+          for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(t, 32 * x + l32, 2 * c + hi), f[c], r16);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[x][i] = !part || ((vis >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
-            top = fmaxf(top, s[x][i]);
-          }
-        }
-        top = fmaxf(m, wave_max32(top));
-        const float ref = top == NEG_INF ? 0.f : top;
-        if (t > 0) {
-          const float keep = fast_exp2(m - ref);
-          sum *= keep;
-          exact *= keep;
-#pragma unroll
-          for (int mt = 0; mt < D / 32; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[mt][i] *= keep;
-        }
-        m = top;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[x][i] = fast_exp2(s[x][i] - ref);
-            exact += s[x][i];
-          }
-          typename O::Frag f[2];
-          operands(s[x], f);
+          for (int i = 0; i < 16; ++i) s[i] = r16[i];
+        };
+        const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            if constexpr (O::ES == 2) {
+            float e[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
-            }
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * x + j, mt, lane), f[j], acc[mt]);
+            for (int i = 0; i < 8; ++i) e[i] = s[8 * j + i];
+            f[j] = O::pack(e);
           }
-        }
-      } else {
+        };
+        if constexpr (!GRAD) {
+          float s[2][16], top = NEG_INF;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float s[16], dp[16];
-          scores(kt, now.q, x, s);
-          scores(vt, now.g, x, dp);
-          const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
+          for (int x = 0; x < 2; ++x) scores(kt, now.q, x, s[x]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float w = fast_exp2(s[i] * a.scale_log2 - now.lse) * (dp[i] - now.delta);
-            s[i] = !part || ((vis >> i) & 1u) ? w : 0.f;
-          }
-          typename O::Frag f[2];
-          operands(s, f);
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) {
-              auto y = T::tr32(kt, 2 * x + j, mt, lane);
-              if constexpr (decltype(careful)::value) y = O::finite(y);
-              acc[mt] = O::mma32(y, f[j], acc[mt]);
+            for (int i = 0; i < 16; ++i) {
+              s[x][i] = !part || ((vis >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
+              top = fmaxf(top, s[x][i]);
             }
+          }
+          top = fmaxf(m, wave_max32(top));
+          const float ref = top == NEG_INF ? 0.f : top;
+          if (t > 0) {
+            const float keep = fast_exp2(m - ref);
+            sum *= keep;
+            exact *= keep;
+#pragma unroll
+            for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[mt][i] *= keep;
+          }
+          m = top;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[x][i] = fast_exp2(s[x][i] - ref);
+              exact += s[x][i];
+            }
+            typename O::Frag f[2];
+            operands(s[x], f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if constexpr (O::ES == 2) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
+              }
+#pragma unroll
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * x + j, mt, lane), f[j], acc[mt]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float s[16], dp[16];
+            scores(kt, now.q, x, s);
+            scores(vt, now.g, x, dp);
+            const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float w = fast_exp2(s[i] * a.scale_log2 - now.lse) * (dp[i] - now.delta);
+              s[i] = !part || ((vis >> i) & 1u) ? w : 0.f;
+            }
+            typename O::Frag f[2];
+            operands(s, f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int mt = 0; mt < D / 32; ++mt) {
+                auto y = T::tr32(kt, 2 * x + j, mt, lane);
+                if constexpr (decltype(careful)::value) y = O::finite(y);
+                acc[mt] = O::mma32(y, f[j], acc[mt]);
+              }
+          }
         }
       }
-    }
     };
     walk(std::false_type{});
     if constexpr (GRAD) {
@@ -1037,176 +1038,176 @@ void by_tile(SArgs a, int hgroups, int tiles_q) {
   bool careful = false, spoilt = false;  // spoilt: some tile held an infinite or NaN value
   for (;; careful = true) {
 #pragma unroll
-  for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
-  m = NEG_INF, sum = 0.f;
-  const int full = GRAD ? min(kSpan, kPos / (4 * R)) : kSpan;
-  for (int lo = 0; lo < blocks; lo += full) {
-    const int span = min(full, blocks - lo);
-    __syncthreads();
-    for (int i = threadIdx.x; i < span * 4; i += 256) (&s_sel[0][0])[i] = 0u;
-    if constexpr (GRAD)
-      for (int i = threadIdx.x; i < span * 4 * R; i += 256) s_pos[i] = -1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 4 * R * p.count; i += 256) {
-      const int t = i / p.count, qq = q0 + t;
-      if (qq >= p.Lq) break;
-      const int c = i % p.count, j = p.blocks[(((int64_t)b * p.Lq + qq) * p.Hkv + hk) * p.count + c] - lo;
-      if (j >= 0 && j < span && (int64_t)(j + lo) * p.block_size < key_limit(p, b, qq, held, start)) {
-        if constexpr (GRAD) {  // (of a repeated block the slot that counts)
-          if (!((a.ok[((int64_t)bh * p.Lq + qq) * a.words + (c >> 5)] >> (c & 31)) & 1u)) continue;
-          s_pos[j * 4 * R + t] = a.pos[((int64_t)bh * p.Lq + qq) * p.count + c];
+    for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
+    m = NEG_INF, sum = 0.f;
+    const int full = GRAD ? min(kSpan, kPos / (4 * R)) : kSpan;
+    for (int lo = 0; lo < blocks; lo += full) {
+      const int span = min(full, blocks - lo);
+      __syncthreads();
+      for (int i = threadIdx.x; i < span * 4; i += 256) (&s_sel[0][0])[i] = 0u;
+      if constexpr (GRAD)
+        for (int i = threadIdx.x; i < span * 4 * R; i += 256) s_pos[i] = -1;
+      __syncthreads();
+      for (int i = threadIdx.x; i < 4 * R * p.count; i += 256) {
+        const int t = i / p.count, qq = q0 + t;
+        if (qq >= p.Lq) break;
+        const int c = i % p.count, j = p.blocks[(((int64_t)b * p.Lq + qq) * p.Hkv + hk) * p.count + c] - lo;
+        if (j >= 0 && j < span && (int64_t)(j + lo) * p.block_size < key_limit(p, b, qq, held, start)) {
+          if constexpr (GRAD) {  // (of a repeated block the slot that counts)
+            if (!((a.ok[((int64_t)bh * p.Lq + qq) * a.words + (c >> 5)] >> (c & 31)) & 1u)) continue;
+            s_pos[j * 4 * R + t] = a.pos[((int64_t)bh * p.Lq + qq) * p.count + c];
+          }
+          atomicOr(&s_sel[j][t / R], 1u << (t % R));
         }
-        atomicOr(&s_sel[j][t / R], 1u << (t % R));
       }
-    }
-    __syncthreads();
-    if (wave == 0) {
-      int n = 0;
-      for (int j = 0; j < span; j += 64) {
-        const bool any = j + lane < span && (s_sel[j + lane][0] | s_sel[j + lane][1] | s_sel[j + lane][2] | s_sel[j + lane][3]);
-        const uint64_t bm = __ballot(any);
-        if (any) s_list[n + __builtin_popcountll(bm & ((1ull << lane) - 1))] = j + lane;
-        n += __builtin_popcountll(bm);
-      }
-      if (lane == 0) s_n = n;
-    }
-    __syncthreads();
-    const int n = __builtin_amdgcn_readfirstlane(s_n);
-    if (n == 0) continue;
-    int e = 0, t = 0;  // tile in flight: entry, tile of its block
-    bool further = false;  // the block has a tile behind it
-    uint32_t bits = 0u;    // the wave's queries that selected the block
-    const auto place = [&]() {
-      const int j = __builtin_amdgcn_readfirstlane(s_list[e]);
-      bits = __builtin_amdgcn_readfirstlane(s_sel[j][wave]);
-      const int64_t k0 = (int64_t)(lo + j) * p.block_size;
-      const int inside = (int)min((int64_t)p.block_size, held - k0);
-      key0 = k0 + t * kKT;
-      key_n = min(inside - t * kKT, kKT);
-      further = t * kKT + kKT < inside;
-      if constexpr (GRAD) {
-        ds_at = live ? s_pos[j * 4 * R + wave * R + qi] : -1;
-        ds_key = t * kKT;
-      }
-    };
-    const auto put = [&](char* kt) {  // the tile in flight to LDS
-      ++seq;
-      char* vt = kt + kKT * T::RB;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = i * RPI + my_r;
-        u32x4 last = GRAD ? xk[i] : xv[GRAD ? 0 : i];
-        if (careful && O::odd(last)) {
-          s_odd[seq & 1] = seq;  // (the other place may still be read for the tile before)
-          last = O::finite16(last);
+      __syncthreads();
+      if (wave == 0) {
+        int n = 0;
+        for (int j = 0; j < span; j += 64) {
+          const bool any = j + lane < span && (s_sel[j + lane][0] | s_sel[j + lane][1] | s_sel[j + lane][2] | s_sel[j + lane][3]);
+          const uint64_t bm = __ballot(any);
+          if (any) s_list[n + __builtin_popcountll(bm & ((1ull << lane) - 1))] = j + lane;
+          n += __builtin_popcountll(bm);
         }
-        if constexpr (!GRAD) *(u32x4*)(kt + T::at(r, my_c)) = xk[i];
-        *(u32x4*)((GRAD ? kt : vt) + T::at(r, my_c)) = last;
+        if (lane == 0) s_n = n;
       }
-      if constexpr (GRAD) {
+      __syncthreads();
+      const int n = __builtin_amdgcn_readfirstlane(s_n);
+      if (n == 0) continue;
+      int e = 0, t = 0;  // tile in flight: entry, tile of its block
+      bool further = false;  // the block has a tile behind it
+      uint32_t bits = 0u;    // the wave's queries that selected the block
+      const auto place = [&]() {
+        const int j = __builtin_amdgcn_readfirstlane(s_list[e]);
+        bits = __builtin_amdgcn_readfirstlane(s_sel[j][wave]);
+        const int64_t k0 = (int64_t)(lo + j) * p.block_size;
+        const int inside = (int)min((int64_t)p.block_size, held - k0);
+        key0 = k0 + t * kKT;
+        key_n = min(inside - t * kKT, kKT);
+        further = t * kKT + kKT < inside;
+        if constexpr (GRAD) {
+          ds_at = live ? s_pos[j * 4 * R + wave * R + qi] : -1;
+          ds_key = t * kKT;
+        }
+      };
+      const auto put = [&](char* kt) {  // the tile in flight to LDS
+        ++seq;
+        char* vt = kt + kKT * T::RB;
 #pragma unroll
-        for (int i = 0; i < kKT / 16; ++i) cs[i] = xs[i];
-      }
-    };
-    place();
-    fetch();
-    put(lds[0]);
-    barrier_lds();
-    int buf = 0;
-    while (e < n) {
-      const char *kt = lds[buf], *vt = kt + kKT * T::RB;
-      const int see = live && ((bits >> qi) & 1u) ? (int)min((int64_t)key_n, lim - key0) : 0;
-      spoilt = spoilt || (careful && s_odd[seq & 1] == seq);
-      if (further) {
-        ++t;
-      } else {
-        ++e;
-        t = 0;
-      }
-      if (e < n) {
-        place();
-        fetch();
-      }
-      if (__any(see > 0)) {
-        const bool slow = !GRAD && (careful || __any(see > 0 && see < kKT));  // some row sees a part of the tile
-        const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int u, float(&s)[16]) {
-          f32x16 r16 = f32x16{};
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(tile, 32 * u + l32, 2 * c + hi), f[c], r16);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = r16[i];
-        };
-        const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = s[8 * j + i];
-            f[j] = O::pack(y);
+        for (int i = 0; i < N; ++i) {
+          const int r = i * RPI + my_r;
+          u32x4 last = GRAD ? xk[i] : xv[GRAD ? 0 : i];
+          if (careful && O::odd(last)) {
+            s_odd[seq & 1] = seq;  // (the other place may still be read for the tile before)
+            last = O::finite16(last);
           }
-        };
-        if constexpr (!GRAD) {
-          float s[2][16];
+          if constexpr (!GRAD) *(u32x4*)(kt + T::at(r, my_c)) = xk[i];
+          *(u32x4*)((GRAD ? kt : vt) + T::at(r, my_c)) = last;
+        }
+        if constexpr (GRAD) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) scores(kt, qf, u, s[u]);
-          if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 6, 1>();
-          if (slow) {
+          for (int i = 0; i < kKT / 16; ++i) cs[i] = xs[i];
+        }
+      };
+      place();
+      fetch();
+      put(lds[0]);
+      barrier_lds();
+      int buf = 0;
+      while (e < n) {
+        const char *kt = lds[buf], *vt = kt + kKT * T::RB;
+        const int see = live && ((bits >> qi) & 1u) ? (int)min((int64_t)key_n, lim - key0) : 0;
+        spoilt = spoilt || (careful && s_odd[seq & 1] == seq);
+        if (further) {
+          ++t;
+        } else {
+          ++e;
+          t = 0;
+        }
+        if (e < n) {
+          place();
+          fetch();
+        }
+        if (__any(see > 0)) {
+          const bool slow = !GRAD && (careful || __any(see > 0 && see < kKT));  // some row sees a part of the tile
+          const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int u, float(&s)[16]) {
+            f32x16 r16 = f32x16{};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t vis = below(see - 32 * u, hi);
+            for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(tile, 32 * u + l32, 2 * c + hi), f[c], r16);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) s[u][i] = mask_neg_inf(s[u][i], seen_bit(vis, i));
-            }
-          }
-          float top = NEG_INF;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[u][i], s[u][i + 1]), top);
-          top = see > 0 ? wave_max32(top) : NEG_INF;  // (both halves of a row have one `see`)
-          if (__any((top - m) * sl > 8.f)) {          // (the first scores of a row: m is -inf)
-            const float to = fmaxf(m, top), keep = to == NEG_INF ? 1.f : fast_exp2((m - to) * sl);
-            m = to;
-            sum *= keep;
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] *= keep;
-          }
-          const float ref = see > 0 ? (m == NEG_INF ? 0.f : m * sl) : -NEG_INF;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = fast_exp2(__builtin_fmaf(s[u][i], sl, -ref));
-            typename O::Frag f[2];
-            operands(s[u], f);
+            for (int i = 0; i < 16; ++i) s[i] = r16[i];
+          };
+          const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              sum = O::total(f[j], sum);
+              float y[8];
 #pragma unroll
-              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * u + j, mt, lane), f[j], acc[mt]);
+              for (int i = 0; i < 8; ++i) y[i] = s[8 * j + i];
+              f[j] = O::pack(y);
             }
+          };
+          if constexpr (!GRAD) {
+            float s[2][16];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) scores(kt, qf, u, s[u]);
+            if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 6, 1>();
+            if (slow) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t vis = below(see - 32 * u, hi);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[u][i] = mask_neg_inf(s[u][i], seen_bit(vis, i));
+              }
+            }
+            float top = NEG_INF;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[u][i], s[u][i + 1]), top);
+            top = see > 0 ? wave_max32(top) : NEG_INF;  // (both halves of a row have one `see`)
+            if (__any((top - m) * sl > 8.f)) {          // (the first scores of a row: m is -inf)
+              const float to = fmaxf(m, top), keep = to == NEG_INF ? 1.f : fast_exp2((m - to) * sl);
+              m = to;
+              sum *= keep;
+#pragma unroll
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] *= keep;
+            }
+            const float ref = see > 0 ? (m == NEG_INF ? 0.f : m * sl) : -NEG_INF;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[u][i] = fast_exp2(__builtin_fmaf(s[u][i], sl, -ref));
+              typename O::Frag f[2];
+              operands(s[u], f);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                sum = O::total(f[j], sum);
+#pragma unroll
+                for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * u + j, mt, lane), f[j], acc[mt]);
+              }
+            }
+            if constexpr (O::ES == 2) reads_ahead<4 * D / 32, 6, 2>();
+          } else {
+#pragma unroll
+            for (int i = 0; i < kKT / 16; ++i)
+#pragma unroll
+              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32n(kt, i, mt, lane), cs[i], acc[mt]);
+            if constexpr (O::ES == 2) reads_ahead<kKT / 16 * D / 32, 6, 2>();
           }
-          if constexpr (O::ES == 2) reads_ahead<4 * D / 32, 6, 2>();
-        } else {
-#pragma unroll
-          for (int i = 0; i < kKT / 16; ++i)
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32n(kt, i, mt, lane), cs[i], acc[mt]);
-          if constexpr (O::ES == 2) reads_ahead<kKT / 16 * D / 32, 6, 2>();
         }
+        if constexpr (NBUF == 2) buf ^= 1;
+        else barrier_lds();  // all are done with the one buffer
+        if (e < n) put(lds[buf]);
+        barrier_lds();
       }
-      if constexpr (NBUF == 2) buf ^= 1;
-      else barrier_lds();  // all are done with the one buffer
-      if (e < n) put(lds[buf]);
-      barrier_lds();
     }
-  }
-  if (careful) break;
-  float worst = 0.f;  // NaN where some result is not finite
+    if (careful) break;
+    float worst = 0.f;  // NaN where some result is not finite
 #pragma unroll
-  for (int mt = 0; mt < D / 32; ++mt)
+    for (int mt = 0; mt < D / 32; ++mt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) worst = __builtin_fmaf(acc[mt][i], 0.f, worst);
-  if (!__syncthreads_or(live && worst != 0.f)) break;
+      for (int i = 0; i < 16; ++i) worst = __builtin_fmaf(acc[mt][i], 0.f, worst);
+    if (!__syncthreads_or(live && worst != 0.f)) break;
   }
 
   const int64_t* os = GRAD ? p.dq_stride : p.o_stride;
@@ -1485,7 +1486,7 @@ int sel_check(const mattn_selected* p) {
   if (p->D <= 0 || p->D > 128 || p->D % 8) return MATTN_ERR_HEAD_DIM;
   if (p->block_size <= 0 || p->block_size % 16 || p->count <= 0 || p->count > kMaxSel) return MATTN_ERR_SHAPE;
   if (p->dtype != MATTN_BF16 && p->dtype != MATTN_F16 && p->dtype != MATTN_F32) return MATTN_ERR_DTYPE;
-  if (!isfinite(p->scale)) return MATTN_ERR_SHAPE;
+  if (!isfinite(p->scale * 1.4426950408889634f)) return MATTN_ERR_SHAPE;
   if (!p->blocks) return MATTN_ERR_NULL;
   const int es = p->dtype == MATTN_F32 ? 4 : 2;
   for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride, p->o_stride, p->do_stride, p->dq_stride, p->dk_stride, p->dv_stride})
@@ -1526,7 +1527,8 @@ SPlan sel_plan(const mattn_selected* p) {
   const bool fits = p->k_stride[1] < (1 << 30) / (64 * es) && p->v_stride[1] < (1 << 30) / (64 * es);
   const bool f32 = p->dtype == MATTN_F32;
   s.tile_fwd = !s.by_query && fits && (f32 ? U < 1.9 * n && T == 1 : U * T < n * (5.4 + 1.9 * T));
-  s.tile_bwd = fits && !f32 && U * T < n * (8.3 + 2.6 * T);
+  // (dS takes 2 block_size bytes a row and block in memory, partial rows 4 D: wide blocks keep to those)
+  s.tile_bwd = fits && !f32 && p->block_size <= kMaxDS && U * T < n * (8.3 + 2.6 * T);
   s.splits = 1;
   while (s.splits < 32 && wgs * s.splits < 512 && tiles / (2 * s.splits) >= 4) s.splits *= 2;
   return s;

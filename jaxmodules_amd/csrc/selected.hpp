@@ -222,12 +222,6 @@ struct STile {
       return o;
     }
   }
-  // an infinite or NaN value among the first `rows` rows (the same answer in all lanes)
-  static __device__ __forceinline__ bool odd(const char* t, int rows, int lane) {
-    bool any = false;
-    for (int i = lane; i < rows * CPR; i += 64) any = any || O::odd(*(const u32x4*)(t + 16 * i));
-    return __any(any);
-  }
 };
 
 }  // namespace mattn

@@ -255,7 +255,7 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks
         (None: i) and sees keys below lengths[b] (None: L; clamped to [0, L]) and, with
         is_causal, up to its own position.  Keys it does not see are not read into its
         result, whatever they hold.
-    scale: of the scores (default 1 / sqrt(d)); finite.
+    scale: of the scores (default 1 / sqrt(d)); finite, below 2e38.
 
     Returns [B, N, Hq, d] in q's dtype; differentiable once w.r.t. q, k and v (blocks,
     starts and lengths must not change before the backward).  A query without a key gives
@@ -277,8 +277,8 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks
         raise NotImplementedError(f"{name}: {blocks.shape[3]} blocks of a query are more than {MAX_COUNT}")
     _check_sequences(name, B, starts=starts, lengths=lengths)
     s = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not abs(s) < 3.4028235677973366e38:
-        raise ValueError(f"{name}: scale must be a finite float32, got {scale}")
+    if not abs(s) < 2e38:  # (times log2 e it has to be a float32)
+        raise ValueError(f"{name}: scale must be finite and below 2e38, got {scale}")
     on_gpu(name, q, k, v, blocks, starts, lengths)
     grads = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if q.numel() == 0 or k.numel() == 0 or blocks.numel() == 0:  # no query, or none with a key

@@ -104,6 +104,13 @@ def test_c_entries_refuse():
         setattr(m, field, was)
 
 
+def test_a_scale_that_is_no_float32_times_log2_e_is_refused():
+    with pytest.raises(ValueError, match="scale"):
+        jm.selected_attention(Q, K, K, BLK, 16, scale=3e38)
+    assert _lib.load().mattn_selected_validate(_struct(scale=3e38)) == -2
+    assert _lib.load().mattn_selected_validate(_struct(scale=-2e38)) == 0
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     import os
     import subprocess

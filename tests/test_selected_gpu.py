@@ -2,6 +2,7 @@
 loops on the CPU (tests/selected_oracle.py, which derives the tolerances)."""
 import math
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -442,3 +443,217 @@ def test_blocks_changed_before_the_backward_are_an_error():
     blocks.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+# ---- calls at the edges ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("N,L,H,bs,count", [(150, 200, 2, 32, 3), (150, 700, 1, 16, 1), (20, 300, 4, 64, 2), (5, 200, 2, 16, 4)])
+def test_padded_batches_with_gradients(N, L, H, bs, count, dtype):
+    """The last N tokens of ragged sequences, some shorter than N or empty: queries before a
+    sequence's start see nothing, and NaN behind its end reaches no gradient."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(N + L)
+    lengths = _ints(L, 77, 16, 0, -5)
+    starts = lengths - N
+    B, d = len(lengths), 64
+    q, do = (_normal(gen, B, N, H, d, dtype=dtype) for _ in range(2))
+    k, v = (_normal(gen, B, L, 1, d, dtype=dtype) for _ in range(2))
+    for b, n in enumerate(lengths.tolist()):
+        k[b, max(n, 0):], v[b, max(n, 0):] = float("nan"), float("nan")
+    x = [t.requires_grad_() for t in (q, k, v)]
+    blocks = _blocks(gen, B, N, 1, count, -(-L // bs))
+    o = jm.selected_attention(*x, blocks, bs, starts=starts, lengths=lengths)
+    grads = torch.autograd.grad(o, x, do)
+    want, top = so.attend(*x, so.visible(blocks, N, L, bs, True, starts, lengths), do=do)
+    _check(o, want["o"], o.dtype, top, d, count * bs, "o")
+    for n, g in zip(("dq", "dk", "dv"), grads):
+        _check(g, want[n], o.dtype, top, d, max(count * bs, N * H), n)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("N", [4, 100])
+@pytest.mark.parametrize("Hq", [3, 5, 33, 40, 64])
+def test_groups_of_any_size(Hq, N, dtype):
+    import jaxmodules_amd as jm
+
+    gen = _gen(Hq)
+    d, bs, L = 64, 16, 120
+    x = [_normal(gen, 1, n, h, d, dtype=dtype).requires_grad_() for n, h in ((N, Hq), (L, 1), (L, 1))]
+    do = _normal(gen, 1, N, Hq, d, dtype=dtype)
+    blocks = _blocks(gen, 1, N, 1, 3, 8)
+    starts = _ints(L - N)
+    o = jm.selected_attention(*x, blocks, bs, starts=starts)
+    want, top = so.attend(*x, so.visible(blocks, N, L, bs, True, starts, None), do=do)
+    _check(o, want["o"], o.dtype, top, d, 48, "o")
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, x, do)):
+        _check(g, want[n], o.dtype, top, d, N * Hq, n)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("bs,count,L", [(1040, 2, 2100), (4096, 1, 300), (1024, 3, 2048), (16, 1024, 500)])
+def test_wide_blocks_and_long_selections(bs, count, L, dtype):
+    import jaxmodules_amd as jm
+
+    gen = _gen(bs + count)
+    N, d = 70, 64
+    x = [_normal(gen, 1, n, h, d, dtype=dtype).requires_grad_() for n, h in ((N, 2), (L, 1), (L, 1))]
+    do = _normal(gen, 1, N, 2, d, dtype=dtype)
+    nblk = -(-L // bs)
+    blocks = _blocks(gen, 1, N, 1, count, nblk)
+    blocks[0, ::7, 0, 0], blocks[0, 1::7, 0, 0] = -2 ** 31, 2 ** 31 - 1
+    for causal in (True, False):
+        starts = _ints(L - N) if causal else None
+        o = jm.selected_attention(*x, blocks, bs, starts=starts, is_causal=causal)
+        want, top = so.attend(*x, so.visible(blocks.clamp(-1, nblk), N, L, bs, causal, starts, None), do=do)
+        _check(o, want["o"], o.dtype, top, d, L, "o")
+        for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, x, do)):
+            _check(g, want[n], o.dtype, top, d, L, n)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("N,bs,count", [(8, 16, 4), (120, 32, 2), (400, 16, 1)])
+def test_keys_expanded_over_the_sequence_or_overlapping(N, bs, count, dtype):
+    """K one row for all keys (stride 0), V rows of 64 that start 8 apart."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(N)
+    L, d = 500, 64
+    q, do = _normal(gen, 1, N, 2, d, dtype=dtype).requires_grad_(), _normal(gen, 1, N, 2, d, dtype=dtype)
+    row = _normal(gen, 1, 1, 2, d, dtype=dtype).requires_grad_()
+    flat = _normal(gen, 2 * (8 * L + d), dtype=dtype)
+    blocks = _blocks(gen, 1, N, 2, count, -(-L // bs))
+    starts = _ints(L - N)
+    res = []
+    for dense in (False, True):
+        k = row.expand(1, L, 2, d)
+        v = flat.as_strided((1, L, 2, d), (0, 8, 8 * L + d, 1)).detach()
+        if dense:
+            k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+        v.requires_grad_()
+        o = jm.selected_attention(q, k, v, blocks, bs, starts=starts)
+        res.append([o, *torch.autograd.grad(o, (q, row, v), do)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_positions_at_the_end_of_int32():
+    import jaxmodules_amd as jm
+
+    gen = _gen(3)
+    q, k, v = (_normal(gen, 1, n, 2, 64, dtype="bfloat16") for n in (30, 200, 200))
+    m = jm.block_means(k, 16)
+    far = _ints(2 ** 31 - 1)
+    sel = jm.select_blocks(q, m, 16, 3, starts=far)
+    assert torch.equal(sel, jm.select_blocks(q, m, 16, 3, is_causal=False))
+    assert torch.equal(jm.selected_attention(q, k, v, sel, 16, starts=far), jm.selected_attention(q, k, v, sel, 16, is_causal=False))
+    none = jm.select_blocks(q, m, 16, 3, starts=-far)
+    assert (none == -1).all()
+    assert not jm.selected_attention(q, k, v, sel, 16, starts=-far).any()
+
+
+@pytest.mark.parametrize("N", [1, 20])
+def test_a_cache_of_more_than_2_31_elements(N):
+    """The newest keys of one long cache: offsets pass 32 bits in means, scores and attention."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(N)
+    H, d, bs, L = 8, 128, 16, 1_100_000
+    cache = torch.empty((1, L, 2, H, d), dtype=torch.bfloat16, device="cuda")  # K and V of a token side by side
+    assert cache.numel() > 2 ** 31
+    tail = 40 * bs  # the keys that are filled
+    cache[:, L - tail - bs:] = 0.0
+    cache[:, L - tail:] = _normal(gen, 1, tail, 2, H, d, dtype="bfloat16")
+    k, v = cache[:, :, 0], cache[:, :, 1]
+    q = _normal(gen, 1, N, 2 * H, d, dtype="bfloat16")
+    lengths, starts = _ints(L), _ints(L - N)
+    nblk = L // bs
+    means = torch.full((1, nblk, H, d), -1.0, device="cuda")
+    jm.block_means(k, bs, lengths, out=means, new=tail)
+    torch.testing.assert_close(means[:, nblk - 40:].double().cpu(), so.means(k[:, L - tail:], bs), rtol=2 ** -23, atol=1e-30)
+    assert (means[:, : nblk - 40] == -1).all()
+    means[:, : nblk - 40] = 0.0  # (scores 0: the best few of the filled ones are above)
+    sel = jm.select_blocks(q, means, bs, 6, starts=starts, lengths=lengths, first=0)
+    want, score = so.select(q, means[:, nblk - 40:], bs, 6, starts=starts - (L - tail), lengths=lengths - (L - tail), first=0)
+    assert (np.sort(score[..., :-2], -1)[..., -5] > 0).all()
+    assert torch.equal((sel - (nblk - 40)).cpu(), want)
+    sel = nblk - 40 + _blocks(gen, 1, N, H, 6, 40)
+    o = jm.selected_attention(q, k, v, sel, bs, starts=starts, lengths=lengths)
+    # (-1 of the draw is the block before the filled ones: the oracle's tail holds it too)
+    own, more = (sel - (nblk - 41)).clamp(-1, 41), tail + bs
+    ref, top = so.attend(q, k[:, L - more:], v[:, L - more:], so.visible(own, N, more, bs, True, starts - (L - more), None))
+    _check(o, ref["o"], o.dtype, top, d, 6 * bs, "o")
+
+
+def test_means_and_choice_of_many_blocks():
+    import jaxmodules_amd as jm
+
+    gen = _gen(8)
+    L, d = 1_100_000, 8
+    k = _normal(gen, 1, L, 1, d, dtype="bfloat16")
+    m = jm.block_means(k, 16)
+    torch.testing.assert_close(m, k.view(1, L // 16, 16, 1, d).double().mean(2).float(), rtol=2 ** -22, atol=1e-30)
+    q = _normal(gen, 1, 3, 2, d, dtype="bfloat16")
+    sel = jm.select_blocks(q, m, 16, 5, is_causal=False, first=0, last=0)
+    score = torch.einsum("bnd,bjd->bnj", q.double().sum(2), m[:, :, 0].double())
+    assert torch.equal(sel[0, :, 0].long(), score[0].topk(5).indices.sort().values)
+
+
+def test_two_streams_at_once():
+    """Calls in flight together on two streams have workspaces of their own."""
+    import jaxmodules_amd as jm
+
+    gen = _gen(21)
+    sets = []
+    for i, (n, bs, count) in enumerate(((2000, 64, 8), (1500, 32, 6))):
+        x = [_normal(gen, 1, n, h, 128, dtype="bfloat16").requires_grad_() for h in (8, 2, 2)]
+        sets.append((x, _normal(gen, 1, n, 8, 128, dtype="bfloat16"), bs, count, torch.cuda.Stream()))
+
+    def step(x, do, bs, count, _):
+        sel = jm.select_blocks(x[0], jm.block_means(x[1], bs), bs, count)
+        o = jm.selected_attention(*x, sel, bs)
+        return [sel, o.detach(), *torch.autograd.grad(o, x, do)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(s[-1]):
+                got[i].append(step(*s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    import jaxmodules_amd as jm
+
+    gen = _gen(22)
+    cases = []
+    for n, lengths in ((1, _ints(700, 90)), (64, _ints(700, 300))):
+        q = _normal(gen, 2, n, 8, 64, dtype="bfloat16")
+        k, v = (_normal(gen, 2, 704, 2, 64, dtype="bfloat16") for _ in range(2))
+        means = jm.block_means(k, 32, lengths)
+
+        def run(q=q, k=k, v=v, means=means, lengths=lengths, n=n):
+            jm.block_means(k, 32, lengths, out=means, new=n)
+            sel = jm.select_blocks(q, means, 32, 6, starts=lengths - n, lengths=lengths)
+            return sel, jm.selected_attention(q, k, v, sel, 32, starts=lengths - n, lengths=lengths)
+
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        cases.append((graph, out, run, (q, k, v), lengths))
+    for i in range(3):
+        for graph, _, _, x, lengths in cases:
+            for t in x:
+                t.copy_(torch.randn_like(t))
+            lengths.add_(1)
+            graph.replay()
+        for _, out, run, _, _ in cases:
+            assert all(torch.equal(a, b) for a, b in zip(out, run())), i
