@@ -265,3 +265,63 @@ def test_side_stream_and_graph():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_odd_addresses_expanded_inputs_and_gradients(dtype):
+    """Weights at an odd address, one row expanded over positions and heads, an upstream
+    gradient of one value: as of dense copies."""
+    import jaxmodules_amd as jm
+
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    dt = getattr(torch, dtype)
+    f, _ = _freq(32)
+    flat = torch.rand(129, generator=gen, device="cuda")
+    row = torch.randn((1, 1, 1, 128), generator=gen, device="cuda").to(dt)
+    pos = torch.arange(90, device="cuda").view(30, 3).t()  # strides (1, 3)
+    res = []
+    for dense in (False, True):
+        fit = (lambda t: t.contiguous().clone()) if dense else (lambda t: t)
+        w = fit(flat[1:]).detach().requires_grad_()
+        x = fit(row.expand(3, 30, 4, 128)).detach().requires_grad_()
+        o = jm.norm_rotary(x, None, w, positions=fit(pos), inv_freq=f, layout="interleaved")
+        up = fit(torch.full((), 0.5, dtype=dt, device="cuda").expand_as(o))
+        res.append([o.detach(), *torch.autograd.grad(o, (x, w), up), jm.rotary(x.detach(), positions=fit(pos), inv_freq=f)])
+    for a, b in zip(*res):  # (one column a load adds in another order than eight)
+        torch.testing.assert_close(a, b, rtol=2 ** -7 if dtype == "bfloat16" else 1e-5, atol=1e-3 if dtype == "bfloat16" else 1e-5)
+
+
+def test_one_token_equals_its_prompt():
+    import jaxmodules_amd as jm
+
+    q, k = _pair(2, 70, 8, 2, 128, "bfloat16", 41)
+    f, scale = _freq(64, scaling="parts", factor=4.0, context=64)
+    w = torch.rand(128, device="cuda")
+    a, b = jm.norm_rotary(q, k, w, w, inv_freq=f, scale=scale)
+    for t in (0, 33, 69):
+        p = torch.full((2, 1), t, dtype=torch.int32, device="cuda")
+        c, d = jm.norm_rotary(q[:, t:t + 1], k[:, t:t + 1], w, w, p, inv_freq=f, scale=scale)
+        assert torch.equal(c[:, 0], a[:, t]) and torch.equal(d[:, 0], b[:, t])
+
+
+def test_two_streams_at_once():
+    import jaxmodules_amd as jm
+
+    f, _ = _freq(64)
+    w = torch.rand(128, device="cuda")
+    sets = [(_pair(1, 3000, 16, 4, 128, "bfloat16", i), _pair(1, 3000, 16, 4, 128, "bfloat16", 9 + i), torch.cuda.Stream()) for i in range(2)]
+
+    def step(x, g, _):
+        x = [t.detach().requires_grad_() for t in (*x, w)]
+        o = jm.norm_rotary(x[0], x[1], x[2], x[2], inv_freq=f)
+        return [t.detach() for t in o] + list(torch.autograd.grad(o, x, g))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(s[-1]):
+                got[i].append(step(*s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for g in got[i] for a, b in zip(g, want[i]))
