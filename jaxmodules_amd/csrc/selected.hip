@@ -6,7 +6,7 @@
 //   delta = dO . O, dS = P (dO . V - delta) scale; dQ = dS K, dK = dS^T Q, dV = P^T dO
 //
 // Two forms.  By blocks (prompts and training): the queries that selected a block are
-// listed once (list_* kernels), and a workgroup takes a block's keys and up to kRows rows
+// listed once (list_* kernels), and a workgroup takes a block's keys and some hundred rows
 // (query, head) of its list: whole matrix-core tiles whatever G is, K and V read once for
 // all of them.  A row's results of its blocks are joined by a second kernel: partial O
 // (and dQ) are float32 rows with a log-sum-exp, at [row][slot of the block in the query's
@@ -35,8 +35,8 @@ constexpr int kChunkQ = 256;    // queries a list workgroup takes
 constexpr int kRange = 1024;    // blocks a list workgroup takes
 constexpr int kSlotBits = 10;   // of a list entry
 constexpr int kMaxSel = 1 << kSlotBits;  // blocks of a query
-constexpr int kRows = 512;      // rows (query, head) of a block that a forward or dQ workgroup takes
-constexpr int kRowsKV = 2048;   // rows that a dK/dV workgroup takes
+constexpr int kRows = 512;      // rows (query, head) of a block that a forward or dQ workgroup takes at most
+constexpr int kRowsKV = 2048;   // rows that a dK/dV workgroup takes at most
 constexpr int kMaxDS = 1024;    // keys of a block whose dS is kept in memory
 
 struct Desc {
@@ -63,6 +63,7 @@ struct SArgs {
   void* ds;                  // [B * Hkv][Lq * count (as ent)][G][block_size] dS / scale, the inputs' type (or null)
   Desc *tile, *kvtile;       // [B * Hkv][max_tiles], [B * Hkv][max_kv]
   int words, chunks, max_tiles, max_kv, subs;  // subs: dK/dV key tiles of a block
+  int rows_q, rows_kv;                         // rows of a work item
 };
 
 __device__ __forceinline__ int keys_held(const mattn_selected& p, int b) {
@@ -180,7 +181,7 @@ void list_items(SArgs a) {
   for (int j0 = 0; j0 < a.nblk; j0 += kScan) {
     const int j = j0 + t, n = j < a.nblk ? off[j] : 0;
     const int rows = n * a.G;
-    const int v[3] = {n, (rows + kRows - 1) / kRows, (rows + kRowsKV - 1) / kRowsKV * a.subs};
+    const int v[3] = {n, (rows + a.rows_q - 1) / a.rows_q, (rows + a.rows_kv - 1) / a.rows_kv * a.subs};
     int s[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -207,7 +208,7 @@ void list_items(SArgs a) {
     // the range's items, a wave a block at a time (values of the wave's own 64 blocks)
     for (int x = 0; x < 64 && j0 + 64 * w + x < a.nblk; ++x) {
       const int nt = __shfl(v[1], x), st = __shfl(s[1], x), nk = __shfl(v[2], x), sk = __shfl(s[2], x);
-      for (int i = lane; i < nt; i += 64) tile[st + i] = Desc{j0 + 64 * w + x, i * kRows};
+      for (int i = lane; i < nt; i += 64) tile[st + i] = Desc{j0 + 64 * w + x, i * a.rows_q};
       // (key tile, rows): the tiles of a block next to each other
       for (int i = lane; i < nk; i += 64) kvtile[sk + i] = Desc{j0 + 64 * w + x, i};
     }
@@ -313,7 +314,7 @@ void by_block_q(SArgs a) {
   if (desc.blk < 0) return;
   const int* off = a.off + (int64_t)bh * (a.nblk + 1) + desc.blk;
   const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
-  const int rows = min((off[1] - off[0]) * a.G - desc.row0, kRows);
+  const int rows = min((off[1] - off[0]) * a.G - desc.row0, a.rows_q);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int held = keys_held(p, b);
   const int64_t start = first_pos(p, b), k0 = (int64_t)desc.blk * p.block_size;
@@ -473,7 +474,7 @@ void by_block_q(SArgs a) {
   }
 }
 
-// dK and dV of a key tile from up to kRowsKV rows: KT keys (64, or 128 for blocks of at
+// dK and dV of a key tile from a.rows_kv rows of its list: KT keys (64, or 128 for blocks of at
 // least 128), 64 rows at a time in LDS.  A wave holds 32 keys (lane = key) as operands in
 // registers and, with KT = 64, every other 32 rows; the scores' result has the rows along
 // its registers, so P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they
@@ -498,9 +499,9 @@ void by_block_kv(SArgs a) {
   if (desc.blk < 0) return;
   const int* off = a.off + (int64_t)bh * (a.nblk + 1) + desc.blk;
   const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
-  const int per = ((off[1] - off[0]) * a.G + kRowsKV - 1) / kRowsKV;  // items of a key tile
-  const int sub = desc.row0 / per, row0 = desc.row0 % per * kRowsKV;
-  const int rows = min((off[1] - off[0]) * a.G - row0, kRowsKV);
+  const int per = ((off[1] - off[0]) * a.G + a.rows_kv - 1) / a.rows_kv;  // items of a key tile
+  const int sub = desc.row0 / per, row0 = desc.row0 % per * a.rows_kv;
+  const int rows = min((off[1] - off[0]) * a.G - row0, a.rows_kv);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int kg = wave % KG, rg = wave / KG;
   const int held = keys_held(p, b);
@@ -1510,25 +1511,31 @@ SPlan sel_plan(const mattn_selected* p) {
   s.hgroups = (int)cdiv(G, 16);
   const int64_t wgs = bh * p->Lq * s.hgroups, tiles = cdiv((int64_t)p->count * p->block_size, 32);
   s.by_query = p->Lq <= 16;
-  // By tiles or by blocks.  A wave's tile holds R queries; where their selections are
-  // independent its union has U = v (1 - (1 - n / v)^R) of the v blocks they see on average
-  // (neighbouring queries share more, which favours tiles).  Measured at D = 128 in 16 bits,
-  // ns: by tiles 1.4 a wave and 64 keys (dQ 1.0, and 0.03 a row for writing dS), by blocks
-  // 0.24 + 0.08 a row and 64 keys (dQ 0.26 + 0.11), 32 rows a wave: at 64 keys a block tiles
-  // up to U = 7.3 n (dQ 11 n), at 512 keys 2.5 n (3.6 n).  [1, 8192, 32/8, 128], 16 blocks of
-  // 64: forward 0.58 ms against 1.36, backward 1.1 against 2.2; [1, 65536, 2, 128]: 2.0 against
-  // 0.81 and 1.9 against 1.3.  Float32 products take eight times as long: forward up to 1.9 n
-  // at 64 keys, dQ by blocks.
+  // By tiles or by blocks, by their times in ns.  A wave's tile holds R queries; where their
+  // selections are independent its union has U = v (1 - (1 - n / v)^R) of the v blocks they see
+  // on average, E of all blocks (neighbouring queries share more, which favours tiles).  Measured
+  // at D = 128 in 16 bits: by tiles 1.4 a wave and 64 keys (dQ 1.0, and 0.03 a row for writing
+  // dS), but no less than a workgroup's walk of E blocks alone takes, 1900 (dQ 1400) for each
+  // 64 keys; by blocks 0.24 + 0.08 a row and 64 keys (dQ 0.26 + 0.11), and some 25 us (dQ 10)
+  // of lists, joining and launches.  At D = 64 0.6 (dQ 0.7) of all that.  Float32 products take
+  // eight times as long; their dQ goes by blocks.  Forward by tiles and by blocks, then both with
+  // their gradients: [1, 8192, 32/8, 128], 16 blocks of 64: 0.62 and 1.38 ms, 1.76 and 3.66; [1,
+  // 6000, 1, 64], 16 of 64: 116 and 73 us, 291 and 133; [1, 8192, 2, 128], 4 of 64: 200 and 74 us;
+  // [1, 300, 8/2, 128], 4 of 64: 21 and 37 us; float32 [1, 1000, 4/1, 128], 9 of 64: 153 and 62 us.
+  const bool f32 = p->dtype == MATTN_F32, narrow = p->D <= 64;
   const double R = G < 32 ? 32 / G : 1, T = (double)cdiv(p->block_size, 64), n = p->count;
-  const double v = fmax(n, (double)cdiv(p->Lk, p->block_size) * (p->causal && !p->starts ? 0.5 : 1.0));
-  const double U = v * (1.0 - pow(1.0 - n / v, R));
-  const int es = p->dtype == MATTN_F32 ? 4 : 2;
+  const double blocks = fmax(n, (double)cdiv(p->Lk, p->block_size)), v = fmax(n, p->causal && !p->starts ? 0.5 * blocks : blocks);
+  const double U = v * (1.0 - pow(1.0 - n / v, R)), E = blocks * (1.0 - pow(1.0 - n / blocks, R));
+  const double rows = (double)bh * p->Lq * G, waves = (double)bh * cdiv(G, 32) * p->Lq / R, m = f32 ? 8.0 : 1.0;
+  const double c = narrow ? 0.6 : 1.0, cb = narrow ? 0.7 : 1.0;
+  const bool tile_fwd = fmax(1.4 * m * waves * U, (f32 ? 9000.0 : 1900.0) * E) * T * c < 25000.0 + rows * n * (0.24 + 0.08 * m * T) * c;
+  const bool tile_bwd = fmax(waves * U, 1400.0 * E) * T * cb + 0.03 * rows * n * T < 10000.0 + rows * n * (0.26 + 0.11 * T) * cb;
+  const int es = f32 ? 4 : 2;
   // (a tile's keys are read through buffers with 32-bit offsets)
   const bool fits = p->k_stride[1] < (1 << 30) / (64 * es) && p->v_stride[1] < (1 << 30) / (64 * es);
-  const bool f32 = p->dtype == MATTN_F32;
-  s.tile_fwd = !s.by_query && fits && (f32 ? U < 1.9 * n && T == 1 : U * T < n * (5.4 + 1.9 * T));
+  s.tile_fwd = !s.by_query && fits && tile_fwd;
   // (dS takes 2 block_size bytes a row and block in memory, partial rows 4 D: wide blocks keep to those)
-  s.tile_bwd = fits && !f32 && p->block_size <= kMaxDS && U * T < n * (8.3 + 2.6 * T);
+  s.tile_bwd = fits && !f32 && p->block_size <= kMaxDS && tile_bwd;
   s.splits = 1;
   while (s.splits < 32 && wgs * s.splits < 512 && tiles / (2 * s.splits) >= 4) s.splits *= 2;
   return s;
@@ -1540,7 +1547,7 @@ struct SLayout {
   // workspace
   size_t cnt, odd, part, plse, fwd;                   // forward
   size_t delta, dqpart, ds, kvpart, bodd, kvodd, bwd;  // backward
-  int words, chunks, nblk, max_tiles, max_kv, subs;
+  int words, chunks, nblk, max_tiles, max_kv, subs, rows_q, rows_kv;
 };
 
 SLayout sel_layout(const mattn_selected* p) {
@@ -1552,8 +1559,16 @@ SLayout sel_layout(const mattn_selected* p) {
   l.subs = (int)cdiv(p->block_size, key_tile(p));
   const int64_t most = (int64_t)p->Lq * p->count;  // entries of a head
   const int64_t used = l.nblk < most ? l.nblk : most;
-  l.max_tiles = (int)(most * G / kRows + used);
-  l.max_kv = (int)((most * G / kRowsKV + used) * l.subs);
+  // fewer rows an item where there would be too few items for the card: at [1, 543, 8, 96] in
+  // float32 over 3 blocks of 256 the step takes 0.28 ms against 0.9
+  const auto share = [&](int64_t of, int64_t unit, int64_t most) {
+    const int64_t x = cdiv(cdiv(of, 1024), unit) * unit;
+    return (int)(x < most ? x : most);
+  };
+  l.rows_q = share(bh * most * G, 128, kRows);
+  l.rows_kv = share(bh * most * G * l.subs, 256, kRowsKV);
+  l.max_tiles = (int)(most * G / l.rows_q + used);
+  l.max_kv = (int)((most * G / l.rows_kv + used) * l.subs);
   size_t x = 0;
   const auto take = [&](size_t bytes) {
     const size_t at = x;
@@ -1599,6 +1614,8 @@ SArgs sel_args(const mattn_selected* p, const SLayout& l, void* lists) {
   a.max_tiles = l.max_tiles;
   a.max_kv = l.max_kv;
   a.subs = l.subs;
+  a.rows_q = l.rows_q;
+  a.rows_kv = l.rows_kv;
   char* c = (char*)lists;
   if (c) {
     a.ok = (uint32_t*)(c + l.ok);
