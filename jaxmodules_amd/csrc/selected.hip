@@ -5,23 +5,28 @@
 //   P_qk = exp(scale q.k - lse_q); the blocks are shared by the G query heads of a key head
 //   delta = dO . O, dS = P (dO . V - delta) scale; dQ = dS K, dK = dS^T Q, dV = P^T dO
 //
-// Two forms.  By blocks (prompts and training): the queries that selected a block are
-// listed once (list_* kernels), and a workgroup takes a block's keys and some hundred rows
-// (query, head) of its list: whole matrix-core tiles whatever G is, K and V read once for
-// all of them.  A row's results of its blocks are joined by a second kernel: partial O
-// (and dQ) are float32 rows with a log-sum-exp, at [row][slot of the block in the query's
-// selection], so that nothing is added in an order of chance.  By queries (few rows, one
-// token of each sequence): a workgroup takes one query and key head, its waves the tiles
-// of 32 keys of its blocks.
+// Three forms (sel_plan).  By queries (few rows, one token of each sequence): a workgroup takes
+// one query and key head, its waves the tiles of 32 keys of its blocks.  By tiles of queries:
+// a wave holds 32 neighbouring rows (query, head) and walks the union of their blocks.  By
+// blocks: the queries that selected a block are listed once (list_* kernels), and a workgroup
+// takes a block's keys and some hundred rows of its list: whole matrix-core tiles whatever the
+// group is, K and V read once for all of them; a row's partial results of its blocks (float32,
+// with a log-sum-exp each, at [row][slot of the block in the query's selection], so that
+// nothing is added in an order of chance) are joined by a second kernel.  dK and dV are always
+// formed by blocks, dQ by tiles (from the dS that the dK/dV kernel leaves in memory) or blocks.
 //
 // Infinite and NaN values: 0 times one is NaN in a matrix product, so a tile with such
 // values in rows that some of its queries (keys) must not see would spoil those.  The
 // products run with such values as 0 and mark the block, and the joining kernels add what
 // they give to the results that do see them, from the formula.
 //
-// Bound by the partial rows (by blocks): D * 4 bytes written and read for each (row,
-// block), 8 times the selected keys' own traffic at G = 4 and 64 keys a block; and by HBM
-// reads of K and V (by queries).
+// Bound by HBM reads of K and V (by queries), by LDS reads and the exponentials beside the
+// matrix products (by tiles, dK/dV), and by the partial rows (by blocks with narrow blocks):
+// D * 4 bytes written and read for each (row, block).  Measured in 16 bits at d = 128:
+// [1, 8192, 32/8], 16 blocks of 64 keys: forward 0.62 ms (union's products at 0.8 PFLOP/s,
+// 3.6 times those of the selections), dK/dV 0.72 ms (0.38 PFLOP/s), dQ 0.42 ms; [1, 16384,
+// 16/4], 4 blocks of 512: 0.43 ms and 0.15 ms of joining (4.2 TB/s); one token of each of 32
+// sequences, 64 blocks of 64: 105 us (5.2 TB/s).
 #include <math.h>
 
 #include <initializer_list>
@@ -221,7 +226,7 @@ void list_items(SArgs a) {
   for (int i = base[2] + t; i < a.max_kv; i += kScan) kvtile[i] = Desc{-1, 0};
 }
 
-// ---- by blocks ------------------------------------------------------------------------
+// ---- by blocks and by tiles: parts of both ----------------------------------------------
 
 // Row r of a block's list: its query, slot and head.
 struct RowId {
@@ -296,18 +301,83 @@ __device__ __forceinline__ uint32_t seen_bit(uint32_t vis, int i) {
 
 constexpr int kKT = 64;  // keys of a staged tile
 
+// One tile of 64 keys for a wave's 32 rows (lane = row, `see` of its keys): scores, the
+// running maximum m (of scores before sl, the positive scale in base 2) and sum, and O.  The
+// scores are formed transposed (rows of the MFMA result: keys), so that a row's softmax is one
+// lane's and its neighbour's, and P^T is the next product's operand as it stands.  The maximum
+// moves only when a score passes it by 2^8 (the weights are then below 2^8, in every type's
+// range), so that the sums are hardly ever rescaled.  The sum adds the weights as rounded to
+// the inputs' type, so that O is a weighted mean of V's rows; its logarithm is the row's lse,
+// here and in the backward.  slow: rows are masked element by element; otherwise one that sees
+// none of the tile gets weights 0 by an infinite subtrahend (NaN where a score is not finite).
+template <class Tag, int D>
+__device__ __forceinline__ void attend_tile(const char* kt, const char* vt, const typename SOp<Tag>::Frag (&qf)[D / 16], int see, bool slow,
+                                            float sl, int lane, float& m, float& sum, f32x16 (&acc)[D / 32]) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  const int l32 = lane & 31, hi = lane >> 5;
+  float s[2][16];  // (single floats: of a 16-register result changed in a branch the compiler has
+                   // written back registers of another value)
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    f32x16 r16 = f32x16{};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(kt, 32 * u + l32, 2 * c + hi), qf[c], r16);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[u][i] = r16[i];
+  }
+  if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 6, 1>();
+  if (slow) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t vis = below(see - 32 * u, hi);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = mask_neg_inf(s[u][i], seen_bit(vis, i));
+    }
+  }
+  float top = NEG_INF;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[u][i], s[u][i + 1]), top);
+  top = see > 0 ? wave_max32(top) : NEG_INF;  // (both halves of a row have one `see`)
+  if (__any((top - m) * sl > 8.f)) {          // (the first scores of a row: m is -inf)
+    const float to = fmaxf(m, top), keep = to == NEG_INF ? 1.f : fast_exp2((m - to) * sl);
+    m = to;
+    sum *= keep;
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt) acc[mt] *= keep;
+  }
+  const float ref = see > 0 ? (m == NEG_INF ? 0.f : m * sl) : -NEG_INF;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[u][i] = fast_exp2(__builtin_fmaf(s[u][i], sl, -ref));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = s[u][8 * j + i];
+      const auto f = O::pack(y);
+      sum = O::total(f, sum);
+#pragma unroll
+      for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * u + j, mt, lane), f, acc[mt]);
+    }
+  }
+  if constexpr (O::ES == 2) reads_ahead<4 * D / 32, 6, 2>();
+}
+
 // Forward and dQ.  Four waves of 32 rows each (lane = row, both halves of a wave), 128 rows
-// at a time; the scores are formed transposed (rows of the MFMA result: keys), so that a
-// row's softmax is one lane's and its neighbour's, and P^T is the next product's operand
-// as it stands.  The first tile of a block of at most 64 keys stays in LDS for all rows.
-// P and dS are rounded to the inputs' type (as V and K are), sums are float32; the sum of
-// the weights adds them as rounded, so that O is a weighted mean of V's rows.
+// at a time.  The tile of a block of at most 64 keys stays in LDS for all rows; of a wider one,
+// forward in 16 bits, the next tile's loads are on their way while this one's products run.
+// P and dS are rounded to the inputs' type (as V and K are), sums are float32.
 template <class Tag, int D, bool GRAD>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(SOp<Tag>::ES == 2 && (D == 64 || !GRAD) ? 2 : 1)))
 void by_block_q(SArgs a) {
   using O = SOp<Tag>;
   using T = STile<Tag, D>;
-  __shared__ __align__(16) char lds[2 * kKT * T::RB];
+  constexpr bool AHEAD = !GRAD && O::ES == 2;
+  __shared__ __align__(16) char lds[AHEAD ? 2 : 1][2 * kKT * T::RB];
   const mattn_selected& p = a.p;
   const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
   const Desc desc = a.tile[(int64_t)bh * a.max_tiles + blockIdx.x / a.bh_n];
@@ -322,8 +392,8 @@ void by_block_q(SArgs a) {
   const int tiles = (inside + kKT - 1) / kKT;
   const char* kb = (const char*)a.k + O::ES * (b * p.k_stride[0] + hk * p.k_stride[2]);
   const char* vb = (const char*)a.v + O::ES * (b * p.v_stride[0] + hk * p.v_stride[2]);
-  char *kt = lds, *vt = lds + kKT * T::RB;
-  bool odd = false;  // GRAD: some tile of K holds an infinite or NaN value
+  const bool zero = p.scale == 0.f;
+  const float sl = zero ? 1.f : fabsf(a.scale_log2);  // (forward: the scale's sign is Q's)
 
   // a row's operands; those of the next 128 rows are loaded ahead of the products of these
   struct Rows {
@@ -342,134 +412,136 @@ void by_block_q(SArgs a) {
       x.delta = a.delta[row];
     }
   };
+  // AHEAD: a tile on its way, this thread's chunks of it
+  constexpr int EC = 16 / O::ES, N = AHEAD ? kKT * T::CPR / 256 : 1, RPI = 256 / T::CPR;
+  const int my_r = threadIdx.x / T::CPR, my_c = threadIdx.x % T::CPR;
+  u32x4 xk[N], xv[N];
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = t * kKT + i * RPI + my_r;
+      const bool in = r < inside && my_c * EC < p.D;
+      xk[i] = in ? *(const u32x4*)(kb + O::ES * ((k0 + r) * p.k_stride[1] + my_c * EC)) : u32x4{0u, 0u, 0u, 0u};
+      xv[i] = in ? *(const u32x4*)(vb + O::ES * ((k0 + r) * p.v_stride[1] + my_c * EC)) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  // the tile on its way to LDS; infinite and NaN values of V as 0, and the block marked
+  const auto put = [&](char* kt) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * RPI + my_r;
+      if (O::odd(xv[i])) {
+        odd = true;
+        xv[i] = O::finite16(xv[i]);
+      }
+      *(u32x4*)(kt + T::at(r, my_c)) = xk[i];
+      *(u32x4*)(kt + kKT * T::RB + T::at(r, my_c)) = xv[i];
+    }
+    if (odd) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
+  };
+
   Rows next;
   load(next, 0);
+  if constexpr (AHEAD) fetch(0);
+  int buf = 0;
+  bool odd = false;  // GRAD: some tile of K holds an infinite or NaN value
   for (int r0 = 0; r0 < rows; r0 += 128) {
     const bool live = r0 + 32 * wave + l32 < rows;
-    const Rows now = next;
+    Rows now = next;
     const RowId id = now.id;
     if (r0 + 128 < rows) load(next, r0 + 128);
     const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
     const int64_t lim = key_limit(p, b, id.q, held, start) - k0;  // keys of the block the row sees
-    const int see = (int)min(lim, (int64_t)inside);
+    const int seen = (int)min(lim, (int64_t)inside);
+    const int64_t out = row * p.count + id.slot;
     f32x16 acc[D / 32];
-    float m, sum, exact;
-    const auto walk = [&](auto careful) {
+    if constexpr (!GRAD) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) now.q[c] = O::sign(now.q[c], p.scale < 0.f, zero);
 #pragma unroll
       for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
-      m = NEG_INF, sum = exact = 0.f;
+      float m = NEG_INF, sum = 0.f;
       for (int t = 0; t < tiles; ++t) {
-        if (tiles > 1 || (r0 == 0 && !decltype(careful)::value)) {
-          __syncthreads();
-          const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
-          const bool vo = stage_keys<Tag, D, kKT, !GRAD>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
-          if (GRAD ? ko : vo) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
-          if constexpr (GRAD) odd = __syncthreads_or(ko) || odd;
-          else __syncthreads();
+        char* kt = lds[buf];
+        if (tiles > 1 || r0 == 0) {
+          if constexpr (AHEAD) {
+            // (the tile before lies in the other buffer, and all were done with this one's last before they came to it)
+            put(kt);
+            barrier_lds();
+            if (tiles > 1) {
+              buf ^= 1;
+              if (t + 1 < tiles || r0 + 128 < rows) fetch(t + 1 < tiles ? t + 1 : 0);
+            }
+          } else {
+            __syncthreads();
+            stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+            if (stage_keys<Tag, D, kKT, true>(kt + kKT * T::RB, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D))
+              a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
+            __syncthreads();
+          }
         }
-        const bool part = __any(see < (t + 1) * kKT);  // some row of the wave does not see all of the tile
-        // S^T of 32 keys: single floats from here on (of a 16-register result changed in a branch
-        // the compiler has written back registers of another value)
-        const auto scores = [&](const char* t, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
-          f32x16 r16 = f32x16{};
+        const int see = min(seen - t * kKT, kKT);
+        if (__any(see > 0)) attend_tile<Tag, D>(kt, kt + kKT * T::RB, now.q, see, __any(see < kKT), sl, lane, m, sum, acc);
+      }
+      sum = wave_sum32(sum);
+      const bool some = sum > 0.f || sum != sum;
+      if (live) {
+        put_row<D>(a.part + out * p.D, acc, some ? 1.f / sum : 0.f, hi, p.D);
+        if (hi == 0) a.plse[out] = some ? __builtin_fmaf(m, sl, __log2f(sum)) : NEG_INF;
+      }
+    } else {
+      char *kt = lds[0], *vt = kt + kKT * T::RB;
+      const auto walk = [&](auto careful) {
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(t, 32 * x + l32, 2 * c + hi), f[c], r16);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = r16[i];
-        };
-        const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = s[8 * j + i];
-            f[j] = O::pack(e);
+        for (int mt = 0; mt < D / 32; ++mt) acc[mt] = f32x16{};
+        for (int t = 0; t < tiles; ++t) {
+          if (tiles > 1 || (r0 == 0 && !decltype(careful)::value)) {
+            __syncthreads();
+            const bool ko = stage_keys<Tag, D, kKT, false>(kt, kb, p.k_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+            stage_keys<Tag, D, kKT, false>(vt, vb, p.v_stride[1], k0 + t * kKT, (int)(k0 + inside), p.D);
+            if (ko) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
+            odd = __syncthreads_or(ko) || odd;
           }
-        };
-        if constexpr (!GRAD) {
-          float s[2][16], top = NEG_INF;
+          const bool part = __any(seen < (t + 1) * kKT);  // some row of the wave does not see all of the tile
+          // S^T of 32 keys, single floats from here on (as in attend_tile)
+          const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
+            f32x16 r16 = f32x16{};
 #pragma unroll
-          for (int x = 0; x < 2; ++x) scores(kt, now.q, x, s[x]);
+            for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(tile, 32 * x + l32, 2 * c + hi), f[c], r16);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              s[x][i] = !part || ((vis >> i) & 1u) ? s[x][i] * a.scale_log2 : NEG_INF;
-              top = fmaxf(top, s[x][i]);
-            }
-          }
-          top = fmaxf(m, wave_max32(top));
-          const float ref = top == NEG_INF ? 0.f : top;
-          if (t > 0) {
-            const float keep = fast_exp2(m - ref);
-            sum *= keep;
-            exact *= keep;
-#pragma unroll
-            for (int mt = 0; mt < D / 32; ++mt)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[mt][i] *= keep;
-          }
-          m = top;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              s[x][i] = fast_exp2(s[x][i] - ref);
-              exact += s[x][i];
-            }
-            typename O::Frag f[2];
-            operands(s[x], f);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if constexpr (O::ES == 2) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += Elt<std::conditional_t<O::ES == 2, Tag, bf16_tag>>::to_f32(elt16(__builtin_bit_cast(u32x4, f[j]), i));
-              }
-#pragma unroll
-              for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * x + j, mt, lane), f[j], acc[mt]);
-            }
-          }
-        } else {
+            for (int i = 0; i < 16; ++i) s[i] = r16[i];
+          };
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             float s[16], dp[16];
             scores(kt, now.q, x, s);
             scores(vt, now.g, x, dp);
-            const uint32_t vis = part ? below(see - t * kKT - 32 * x, hi) : 0xffffu;
+            const uint32_t vis = part ? below(seen - t * kKT - 32 * x, hi) : 0xffffu;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float w = fast_exp2(s[i] * a.scale_log2 - now.lse) * (dp[i] - now.delta);
               s[i] = !part || ((vis >> i) & 1u) ? w : 0.f;
             }
-            typename O::Frag f[2];
-            operands(s, f);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j) {
+              float e[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) e[i] = s[8 * j + i];
+              const auto f = O::pack(e);
 #pragma unroll
               for (int mt = 0; mt < D / 32; ++mt) {
                 auto y = T::tr32(kt, 2 * x + j, mt, lane);
                 if constexpr (decltype(careful)::value) y = O::finite(y);
-                acc[mt] = O::mma32(y, f[j], acc[mt]);
+                acc[mt] = O::mma32(y, f, acc[mt]);
               }
+            }
           }
         }
-      }
-    };
-    walk(std::false_type{});
-    if constexpr (GRAD) {
+      };
+      walk(std::false_type{});
       if (odd) walk(std::true_type{});
-    }
-    const int64_t out = row * p.count + id.slot;
-    if constexpr (GRAD) {
       if (live) put_row<D>(a.part + out * p.D, acc, p.scale, hi, p.D);
-    } else {
-      exact = wave_sum32(exact);
-      sum = O::ES == 2 ? wave_sum32(sum) : exact;
-      if (live) {
-        put_row<D>(a.part + out * p.D, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, hi, p.D);
-        if (hi == 0) a.plse[out] = exact > 0.f || exact != exact ? m + __log2f(exact) : NEG_INF;
-      }
     }
   }
 }
@@ -948,16 +1020,13 @@ void join_keys(SArgs a, int KT) {
 // key head with all their heads), a workgroup four such; it walks the blocks that any of its
 // queries selected, each row masked to its own.  The union grows with the queries of a tile,
 // but no faster than their selections together, and each block costs products (and one read
-// of K and V from the cache) where the form by blocks costs 8 D bytes of memory a row: below
-// (sel_plan).  K and V of the next tile are loaded while this tile's products run.
+// of K and V from the cache) where the form by blocks costs 8 D bytes of memory a row.  K and
+// V of the next tile are loaded while this tile's products run.
 //
-// lane = row, as in by_block_q.  The running maximum moves only when a score passes it by
-// 2^8 (the weights are then below 2^8, in every type's range), so that the accumulators
-// are hardly ever rescaled; a negative or zero scale is folded into Q.  A row that did not
-// select a block gets weights 0 by an infinite subtrahend; where infinite or NaN values make
-// that NaN, or spoil a product (0 times them), the result is not finite, and the workgroup
-// walks its blocks once more with every element masked and such values as 0 (add_odd_keys
-// then gives them to the rows that see them).
+// A negative or zero scale is folded into Q.  A row that did not select a block gets weights 0
+// (attend_tile); where infinite or NaN values make that NaN, or spoil a product (0 times them),
+// the result is not finite, and the workgroup walks its blocks once more with every element
+// masked and such values as 0 (add_odd_keys then gives them to the rows that see them).
 //
 // GRAD: dQ = scale dS K the same way, from the dS that the dK/dV kernel has left in memory:
 // 2 bytes a pair, where a partial row of dQ takes 8 D for each row and block.
@@ -1130,64 +1199,9 @@ void by_tile(SArgs a, int hgroups, int tiles_q) {
           fetch();
         }
         if (__any(see > 0)) {
-          const bool slow = !GRAD && (careful || __any(see > 0 && see < kKT));  // some row sees a part of the tile
-          const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int u, float(&s)[16]) {
-            f32x16 r16 = f32x16{};
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) r16 = O::mma32(T::row(tile, 32 * u + l32, 2 * c + hi), f[c], r16);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = r16[i];
-          };
-          const auto operands = [&](const float(&s)[16], typename O::Frag(&f)[2]) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float y[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] = s[8 * j + i];
-              f[j] = O::pack(y);
-            }
-          };
           if constexpr (!GRAD) {
-            float s[2][16];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) scores(kt, qf, u, s[u]);
-            if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 6, 1>();
-            if (slow) {
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint32_t vis = below(see - 32 * u, hi);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[u][i] = mask_neg_inf(s[u][i], seen_bit(vis, i));
-              }
-            }
-            float top = NEG_INF;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(s[u][i], s[u][i + 1]), top);
-            top = see > 0 ? wave_max32(top) : NEG_INF;  // (both halves of a row have one `see`)
-            if (__any((top - m) * sl > 8.f)) {          // (the first scores of a row: m is -inf)
-              const float to = fmaxf(m, top), keep = to == NEG_INF ? 1.f : fast_exp2((m - to) * sl);
-              m = to;
-              sum *= keep;
-#pragma unroll
-              for (int mt = 0; mt < D / 32; ++mt) acc[mt] *= keep;
-            }
-            const float ref = see > 0 ? (m == NEG_INF ? 0.f : m * sl) : -NEG_INF;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) s[u][i] = fast_exp2(__builtin_fmaf(s[u][i], sl, -ref));
-              typename O::Frag f[2];
-              operands(s[u], f);
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                sum = O::total(f[j], sum);
-#pragma unroll
-                for (int mt = 0; mt < D / 32; ++mt) acc[mt] = O::mma32(T::tr32(vt, 2 * u + j, mt, lane), f[j], acc[mt]);
-              }
-            }
-            if constexpr (O::ES == 2) reads_ahead<4 * D / 32, 6, 2>();
+            const bool slow = careful || __any(see > 0 && see < kKT);  // some row sees a part of the tile
+            attend_tile<Tag, D>(kt, vt, qf, see, slow, sl, lane, m, sum, acc);
           } else {
 #pragma unroll
             for (int i = 0; i < kKT / 16; ++i)
@@ -1516,19 +1530,20 @@ SPlan sel_plan(const mattn_selected* p) {
   // on average, E of all blocks (neighbouring queries share more, which favours tiles).  Measured
   // at D = 128 in 16 bits: by tiles 1.4 a wave and 64 keys (dQ 1.0, and 0.03 a row for writing
   // dS), but no less than a workgroup's walk of E blocks alone takes, 1900 (dQ 1400) for each
-  // 64 keys; by blocks 0.24 + 0.08 a row and 64 keys (dQ 0.26 + 0.11), and some 25 us (dQ 10)
-  // of lists, joining and launches.  At D = 64 0.6 (dQ 0.7) of all that.  Float32 products take
-  // eight times as long; their dQ goes by blocks.  Forward by tiles and by blocks, then both with
-  // their gradients: [1, 8192, 32/8, 128], 16 blocks of 64: 0.62 and 1.38 ms, 1.76 and 3.66; [1,
-  // 6000, 1, 64], 16 of 64: 116 and 73 us, 291 and 133; [1, 8192, 2, 128], 4 of 64: 200 and 74 us;
-  // [1, 300, 8/2, 128], 4 of 64: 21 and 37 us; float32 [1, 1000, 4/1, 128], 9 of 64: 153 and 62 us.
+  // 64 keys; by blocks 0.28 + 0.05 a row and 64 keys (dQ 0.26 + 0.11), and some 25 us (dQ 10)
+  // of lists, joining and launches.  At D = 64 0.6 (dQ 0.7) of all that.  Float32 takes 11 and
+  // 0.64; its dQ goes by blocks.  Forward by tiles and by blocks, then both with their gradients:
+  // [1, 8192, 32/8, 128], 16 blocks of 64: 0.62 and 1.38 ms, 1.76 and 3.66; [1, 6000, 1, 64], 16 of
+  // 64: 116 and 73 us, 291 and 133; [1, 8192, 2, 128], 4 of 64: 200 and 74 us; [1, 300, 8/2, 128],
+  // 4 of 64: 21 and 37 us; float32 [1, 1000, 4/1, 128], 9 of 64: 153 and 62 us.
   const bool f32 = p->dtype == MATTN_F32, narrow = p->D <= 64;
   const double R = G < 32 ? 32 / G : 1, T = (double)cdiv(p->block_size, 64), n = p->count;
   const double blocks = fmax(n, (double)cdiv(p->Lk, p->block_size)), v = fmax(n, p->causal && !p->starts ? 0.5 * blocks : blocks);
   const double U = v * (1.0 - pow(1.0 - n / v, R)), E = blocks * (1.0 - pow(1.0 - n / blocks, R));
-  const double rows = (double)bh * p->Lq * G, waves = (double)bh * cdiv(G, 32) * p->Lq / R, m = f32 ? 8.0 : 1.0;
+  const double rows = (double)bh * p->Lq * G, waves = (double)bh * cdiv(G, 32) * p->Lq / R;
   const double c = narrow ? 0.6 : 1.0, cb = narrow ? 0.7 : 1.0;
-  const bool tile_fwd = fmax(1.4 * m * waves * U, (f32 ? 9000.0 : 1900.0) * E) * T * c < 25000.0 + rows * n * (0.24 + 0.08 * m * T) * c;
+  const bool tile_fwd = fmax((f32 ? 11.0 : 1.4) * waves * U, (f32 ? 9000.0 : 1900.0) * E) * T * c <
+                        25000.0 + rows * n * (0.28 + (f32 ? 0.64 : 0.05) * T) * c;
   const bool tile_bwd = fmax(waves * U, 1400.0 * E) * T * cb + 0.03 * rows * n * T < 10000.0 + rows * n * (0.26 + 0.11 * T) * cb;
   const int es = f32 ? 4 : 2;
   // (a tile's keys are read through buffers with 32-bit offsets)
