@@ -1,7 +1,9 @@
 """MI355X (gfx950) implementation of jaxmodules' masked attention hot path.
 
 ``masked_attention_via_map`` and the ``block_mask`` machinery, forward and
-backward, on hand-written HIP kernels behind the C ABI in ``include/mattn.h``.
+backward, on hand-written HIP kernels behind the C ABI in ``include/mattn.h``;
+beside it rotary positions and head norms (``rotary``) and attention over key
+blocks that the data select (``selected``).
 """
 from . import block_mask, blockmap, masks
 from .attention import (default_kernel, flex_attention, flex_attention_slow, kernel_scale,

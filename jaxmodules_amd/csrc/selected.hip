@@ -24,9 +24,9 @@
 // matrix products (by tiles, dK/dV), and by the partial rows (by blocks with narrow blocks):
 // D * 4 bytes written and read for each (row, block).  Measured in 16 bits at d = 128:
 // [1, 8192, 32/8], 16 blocks of 64 keys: forward 0.62 ms (union's products at 0.8 PFLOP/s,
-// 3.6 times those of the selections), dK/dV 0.72 ms (0.38 PFLOP/s), dQ 0.42 ms; [1, 16384,
+// 3.6 times those of the selections), dK/dV 0.72 ms (0.36 PFLOP/s), dQ 0.42 ms; [1, 16384,
 // 16/4], 4 blocks of 512: 0.43 ms and 0.15 ms of joining (4.2 TB/s); one token of each of 32
-// sequences, 64 blocks of 64: 105 us (5.2 TB/s).
+// sequences, 64 blocks of 64: 105 us (5.1 TB/s).
 #include <math.h>
 
 #include <initializer_list>
