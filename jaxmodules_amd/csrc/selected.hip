@@ -796,6 +796,241 @@ void by_block_kv(SArgs a) {
   }
 }
 
+// The same for 16-bit inputs: eight waves, 64 keys, 128 rows at a time.  A wave forms P and dS
+// of 32 rows and 32 keys (its keys' operands in registers) and leaves them in LDS as the
+// operands of the second products, of which each wave takes 32 columns of dV or dK: the sums
+// of a wave are 32 registers where by_block_kv's are 128, so that two waves fit a SIMD and one
+// waits while the other works.
+template <class Tag, int D, bool DS>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2)))
+void by_block_kv16(SArgs a) {
+  using O = SOp<Tag>;
+  using T = STile<Tag, D>;
+  constexpr int NR = 128, KT = 64, MT = D / 32, NK = MT / 2;  // NK: key groups a wave sums (8 waves: 2 kinds, MT columns, 2 / NK)
+  constexpr int DSB = KT * 2 + 16;  // bytes of a staged row of dS (16 more: rows start on other banks)
+  __shared__ __align__(16) char lds[2 * NR * T::RB];
+  __shared__ u32x4 s_k[2][D / 16][64];         // K's operands (V's are in registers): key group, step, lane
+  __shared__ u32x4 s_f[2][NR / 32][2][2][64];  // P, dS: row group, key group, half, lane
+  __shared__ __align__(16) char s_ds[DS ? NR * DSB : 16];
+  __shared__ __align__(16) float s_lse[NR], s_delta[NR];
+  __shared__ __align__(16) int s_see[NR];
+  __shared__ int64_t s_q[2][NR], s_g[2][NR];
+  const mattn_selected& p = a.p;
+  const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int64_t item = (int64_t)bh * a.max_kv + blockIdx.x / a.bh_n;
+  const Desc desc = a.kvtile[item];
+  if (desc.blk < 0) return;
+  const int* off = a.off + (int64_t)bh * (a.nblk + 1) + desc.blk;
+  const int* list = a.ent + (int64_t)bh * p.Lq * p.count + off[0];
+  const int per = ((off[1] - off[0]) * a.G + a.rows_kv - 1) / a.rows_kv;  // items of a key tile
+  const int sub = desc.row0 / per, row0 = desc.row0 % per * a.rows_kv;
+  const int rows = min((off[1] - off[0]) * a.G - row0, a.rows_kv);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+  const int held = keys_held(p, b);
+  const int64_t start = first_pos(p, b), k0 = (int64_t)desc.blk * p.block_size + sub * KT;
+  const int inside = (int)max(min((int64_t)min(p.block_size - sub * KT, KT), held - k0), (int64_t)0);  // keys of the tile
+  const int xg = wave >> 1, kg = wave & 1, key = 32 * kg + l32;                                       // first products
+  const int kind = wave >> 2, mt = wave % 4 * NK / 2, kg0 = NK == 2 ? 0 : wave & 1;                   // second ones: dV, dK
+  char *qt = lds, *gt = lds + NR * T::RB;
+
+  typename O::Frag vf[D / 16];
+  {
+    typename O::Frag kf[D / 16];
+    if (key < inside) load_rows<Tag, D>(kf, a.k, b * p.k_stride[0] + hk * p.k_stride[2] + (k0 + key) * p.k_stride[1], hi, p.D);
+    if (xg == 0) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) s_k[kg][c][lane] = key < inside ? kf[c] : O::zero();
+    }
+  }
+  if (key < inside) {
+    load_rows<Tag, D>(vf, a.v, b * p.v_stride[0] + hk * p.v_stride[2] + (k0 + key) * p.v_stride[1], hi, p.D);
+  } else {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) vf[c] = O::zero();
+  }
+  f32x16 acc[NK];
+
+  // rows on their way, as in by_block_kv
+  constexpr int N = NR * T::CPR / 512;
+  u32x4 xq[N], xg_[N];
+  // thread r < NR: list entry and head of row r of the stage whose places (ids) come next, what
+  // goes to LDS with the next stage's values, and with those of the stage after it
+  struct Side {
+    float lse, delta;
+    int see;
+  } side{}, later{};
+  int entry = 0, e_at = 0, g_at = 0, r_at = 0;
+  const int last_e = (row0 + rows - 1) / a.G, step_e = NR / a.G, step_g = NR % a.G;
+  const auto ids = [&](int buf) {
+    if (threadIdx.x < NR) {
+      const int r = threadIdx.x, q = entry >> kSlotBits, h = hk * a.G + g_at;
+      const int64_t row = ((int64_t)bh * p.Lq + q) * a.G + g_at;
+      s_q[buf][r] = b * p.q_stride[0] + q * p.q_stride[1] + h * p.q_stride[2];
+      s_g[buf][r] = b * p.do_stride[0] + q * p.do_stride[1] + h * p.do_stride[2];
+      later.lse = a.lse[row];
+      later.delta = a.delta[row];
+      later.see = r_at < rows ? (int)min(max((int64_t)key_limit(p, b, q, held, start) - k0, (int64_t)0), (int64_t)inside) : 0;
+      r_at += NR;
+      e_at += step_e;
+      g_at += step_g;
+      if (g_at >= a.G) {
+        g_at -= a.G;
+        ++e_at;
+      }
+      entry = list[min(e_at, last_e)];
+    }
+  };
+  const auto fetch = [&](int r0, int buf, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = i * 512 + tid, r = x / T::CPR, c = x % T::CPR;
+      const bool live = r0 + r < rows && c * 8 < p.D;
+      xq[i] = live ? *(const u32x4*)((const char*)a.q + 2 * (s_q[buf][r] + c * 8)) : u32x4{0u, 0u, 0u, 0u};
+      xg_[i] = live ? *(const u32x4*)((const char*)a.dO + 2 * (s_g[buf][r] + c * 8)) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  const auto stage = [&](int r0, int buf, bool careful) {  // buf: of the next stage's ids
+    // (opaque: places in LDS worked out ahead of the loop would take the registers of the operands)
+    int tid = threadIdx.x;
+    asm("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5, key = 32 * kg + l32;
+    barrier_lds();  // the stage before is done with the tiles
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = i * 512 + tid, r = x / T::CPR, c = x % T::CPR;
+      *(u32x4*)(qt + T::at(r, c)) = xq[i];
+      *(u32x4*)(gt + T::at(r, c)) = xg_[i];
+    }
+    if (threadIdx.x < NR) {
+      s_lse[threadIdx.x] = side.lse;
+      s_delta[threadIdx.x] = side.delta;
+      s_see[threadIdx.x] = side.see;
+    }
+    side = later;
+    barrier_lds();
+    if (r0 + NR < rows) fetch(r0 + NR, buf, tid);
+    const int groups = min(NR / 32, (rows - r0 + 31) / 32);  // of 32 rows
+    if (xg < groups) {
+      float s[16], dp[16];
+      {
+        f32x16 x16 = f32x16{}, y16 = f32x16{};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) x16 = O::mma32(T::row(qt, 32 * xg + l32, 2 * c + hi), s_k[kg][c][lane], x16);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) y16 = O::mma32(T::row(gt, 32 * xg + l32, 2 * c + hi), vf[c], y16);
+        reads_ahead<D / 16, 3, 2>();
+        reads_ahead<D / 16, 4, 1>();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i] = x16[i];
+          dp[i] = y16[i];
+        }
+      }
+      const bool part = __any(s_see[32 * xg + l32] < KT);  // some row does not see all of the tile
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 32 * xg + 8 * j + 4 * hi;
+        const f32x4 l = *(const f32x4*)(s_lse + r), d = *(const f32x4*)(s_delta + r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = fast_exp2(__builtin_fmaf(s[4 * j + i], a.scale_log2, -l[i])), g = w * (dp[4 * j + i] - d[i]);
+          s[4 * j + i] = w;
+          dp[4 * j + i] = g;
+        }
+      }
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 n = *(const u32x4*)(s_see + 32 * xg + 8 * j + 4 * hi);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t on = key < (int)n[i] ? 0xffffffffu : 0u;
+            asm("" : "+v"(on));
+            s[4 * j + i] = mask_zero(s[4 * j + i], on);
+            dp[4 * j + i] = mask_zero(dp[4 * j + i], on);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float e[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = s[8 * j + i];
+          y[i] = dp[8 * j + i];
+        }
+        const u32x4 df = O::pack(y);
+        s_f[0][xg][kg][j][lane] = O::pack(e);
+        s_f[1][xg][kg][j][lane] = df;
+        if constexpr (DS) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *(uint16_t*)(s_ds + (32 * xg + 16 * j + 8 * (i >> 2) + 4 * hi + (i & 3)) * DSB + key * 2) = (uint16_t)elt16(df, i);
+        }
+      }
+    }
+    barrier_lds();
+    if (r0 + 2 * NR < rows) ids(buf ^ 1);
+    const char* t = kind ? qt : gt;
+    for (int x = 0; x < groups; ++x) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        auto y = T::tr32(t, 2 * x + j, mt, lane);
+        if (careful) y = O::finite(y);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) acc[n] = O::mma32(y, s_f[kind][x][kg0 + n][j][lane], acc[n]);
+      }
+    }
+    if constexpr (DS) {  // dS to memory, past the caches: the rows lie in them
+      const int keys = min(KT, p.block_size - sub * KT) / 8;  // chunks of a row
+      char* o = (char*)a.ds + 2 * ((((int64_t)bh * p.Lq * p.count + off[0]) * a.G + row0 + r0) * p.block_size + sub * KT);
+#pragma unroll
+      for (int i = 0; i < NR * (KT / 8) / 512; ++i) {
+        const int x = i * 512 + tid, r = x / (KT / 8), c = x % (KT / 8);
+        if (r0 + r < rows && c < keys) 
+          __builtin_nontemporal_store(*(const u32x4*)(s_ds + r * DSB + 16 * c), (u32x4*)(o + (int64_t)r * p.block_size * 2 + 16 * c));
+      }
+    }
+  };
+  const auto walk = [&](bool careful) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) acc[n] = f32x16{};
+    r_at = threadIdx.x;
+    const int at = row0 + min((int)threadIdx.x, rows - 1);
+    e_at = at / a.G;
+    g_at = at % a.G;
+    if (threadIdx.x < NR) entry = list[e_at];
+    ids(0);
+    side = later;
+    if (NR < rows) ids(1);
+    __syncthreads();
+    fetch(0, 0, threadIdx.x);
+    for (int r0 = 0, buf = 1; r0 < rows; r0 += NR, buf ^= 1) stage(r0, buf, careful);
+  };
+  walk(false);
+  float worst = 0.f;  // NaN where some result is not finite: as in by_block_kv
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) worst = __builtin_fmaf(acc[n][i], 0.f, worst);
+  if (__syncthreads_or(worst != 0.f)) {
+    a.kvodd[(int64_t)bh * a.nblk + desc.blk] = 1;
+    walk(true);
+  }
+  // kvpart holds dK, then dV
+  float* out = a.kvpart + (item * 2 + (kind ? 0 : 1)) * KT * p.D;
+  const float sc = kind ? p.scale : 1.f;
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 32 * mt + 8 * j + 4 * hi;
+      if (c < p.D)
+        *(f32x4*)(out + (int64_t)(32 * (kg0 + n) + l32) * p.D + c) =
+            f32x4{acc[n][4 * j] * sc, acc[n][4 * j + 1] * sc, acc[n][4 * j + 2] * sc, acc[n][4 * j + 3] * sc};
+    }
+}
+
 // ---- joining --------------------------------------------------------------------------
 
 // whether x holds in some lane of this lane's group of lpr
@@ -1786,6 +2021,10 @@ extern "C" int mattn_selected_bwd(const mattn_selected* p, const void* q, const 
       constexpr int D = decltype(dim)::value;
       if (!s.tile_bwd) hipLaunchKernelGGL((by_block_q<Tag, D, true>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
       const auto kv = [&](auto kt, auto ds) {
+        if constexpr (decltype(kt)::value == 64 && !std::is_same_v<Tag, float>) {
+          hipLaunchKernelGGL((by_block_kv16<Tag, D, decltype(ds)::value>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(512), 0, st, a);
+          return;
+        }
         hipLaunchKernelGGL((by_block_kv<Tag, D, decltype(kt)::value, decltype(ds)::value>), dim3((uint32_t)(a.bh_n * l.max_kv)),
                            dim3(256), 0, st, a);
       };
