@@ -24,7 +24,7 @@
 // matrix products (by tiles, dK/dV), and by the partial rows (by blocks with narrow blocks):
 // D * 4 bytes written and read for each (row, block).  Measured in 16 bits at d = 128:
 // [1, 8192, 32/8], 16 blocks of 64 keys: forward 0.62 ms (union's products at 0.8 PFLOP/s,
-// 3.6 times those of the selections), dK/dV 0.72 ms (0.36 PFLOP/s), dQ 0.42 ms; [1, 16384,
+// 3.6 times those of the selections), dK/dV 0.65 ms (0.40 PFLOP/s), dQ 0.42 ms; [1, 16384,
 // 16/4], 4 blocks of 512: 0.43 ms and 0.15 ms of joining (4.2 TB/s); one token of each of 32
 // sequences, 64 blocks of 64: 105 us (5.1 TB/s).
 #include <math.h>
@@ -546,15 +546,15 @@ void by_block_q(SArgs a) {
   }
 }
 
-// dK and dV of a key tile from a.rows_kv rows of its list: KT keys (64, or 128 for blocks of at
-// least 128), 64 rows at a time in LDS.  A wave holds 32 keys (lane = key) as operands in
-// registers and, with KT = 64, every other 32 rows; the scores' result has the rows along
-// its registers, so P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they
-// stand.  Float32 partial sums per item; the items of a block are added in order.
-// DS: dS also goes to memory, rows of block_size keys in the order of the list, through LDS.
-template <class Tag, int D, int KT, bool DS>
+// dK and dV of a key tile from a.rows_kv rows of its list, float32: KT keys (64, or 128 for
+// blocks of at least 128), 64 rows at a time in LDS.  A wave holds 32 keys (lane = key) as
+// operands in registers and, with KT = 64, every other 32 rows; the scores' result has the rows
+// along its registers, so P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they
+// stand.  Partial sums per item; the items of a block are added in order.
+template <int D, int KT>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
 void by_block_kv(SArgs a) {
+  using Tag = float;
   using O = SOp<Tag>;
   using T = STile<Tag, D>;
   constexpr int NR = 64, KG = KT / 32, RG = 4 / KG;
@@ -562,8 +562,6 @@ void by_block_kv(SArgs a) {
   __shared__ __align__(16) float s_lse[NR], s_delta[NR];
   __shared__ __align__(16) int s_see[NR];
   __shared__ int64_t s_q[NR], s_g[NR];
-  constexpr int DSB = KT * O::ES + 16;  // bytes of a staged row of dS (16 more: rows start on other banks)
-  __shared__ __align__(16) char s_ds[DS ? NR * DSB : 16];
   const mattn_selected& p = a.p;
   const int bh = blockIdx.x % a.bh_n, b = bh / p.Hkv, hk = bh % p.Hkv;
   const int64_t item = (int64_t)bh * a.max_kv + blockIdx.x / a.bh_n;
@@ -628,23 +626,15 @@ void by_block_kv(SArgs a) {
       w.g[i] = live ? *(const u32x4*)((const char*)a.dO + O::ES * (s_g[r] + c * EC)) : u32x4{0u, 0u, 0u, 0u};
     }
   };
-  const auto put_ds = [&](int r0) {  // rows r0 .. r0 + NR - 1
-    if constexpr (DS) {
-      const int keys = min(KT, p.block_size - sub * KT) * O::ES / 16;  // chunks of a row
-      char* o = (char*)a.ds + O::ES * ((((int64_t)bh * p.Lq * p.count + off[0]) * a.G + row0 + r0) * p.block_size + sub * KT);
-#pragma unroll
-      for (int i = 0; i < NR * (KT * O::ES / 16) / 256; ++i) {
-        const int x = i * 256 + threadIdx.x, r = x / (KT * O::ES / 16), c = x % (KT * O::ES / 16);
-        if (r0 + r < rows && c < keys) *(u32x4*)(o + (int64_t)r * p.block_size * O::ES + 16 * c) = *(const u32x4*)(s_ds + r * DSB + 16 * c);
-      }
-    }
-  };
   const auto stage = [&](Stage& w, int r0, auto careful) {
+    // (opaque: places in LDS worked out ahead of the loop would take the registers of the operands)
+    int tid = threadIdx.x;
+    asm("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5, key = 32 * kg + l32;
     barrier_lds();  // the stage before is done with the tiles, all have read the ids
-    if (r0 > 0) put_ds(r0 - NR);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int x = i * 256 + threadIdx.x, r = x / T::CPR, c = x % T::CPR;
+      const int x = i * 256 + tid, r = x / T::CPR, c = x % T::CPR;
       *(u32x4*)(qt + T::at(r, c)) = w.q[i];
       *(u32x4*)(gt + T::at(r, c)) = w.g[i];
     }
@@ -668,7 +658,6 @@ void by_block_kv(SArgs a) {
         for (int c = 0; c < D / 16; ++c) x16 = O::mma32(T::row(qt, 32 * x + l32, 2 * c + hi), kf[c], x16);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) y16 = O::mma32(T::row(gt, 32 * x + l32, 2 * c + hi), vf[c], y16);
-        if constexpr (O::ES == 2) reads_ahead<2 * D / 16, 4, 1>();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[i] = x16[i];
@@ -712,14 +701,6 @@ void by_block_kv(SArgs a) {
         pf[j] = O::pack(e);
         df[j] = O::pack(y);
       }
-      if constexpr (DS) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          char* at = s_ds + (32 * x + 8 * (i >> 2) + 4 * hi + (i & 3)) * DSB + key * O::ES;
-          if constexpr (O::ES == 4) *(float*)at = dp[i];
-          else *(uint16_t*)at = (uint16_t)elt16(__builtin_bit_cast(u32x4, df[i >> 3]), i & 7);
-        }
-      }
       const auto add = [&](f32x16(&acc)[D / 32], const char* t, const typename O::Frag(&f)[2]) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -729,7 +710,6 @@ void by_block_kv(SArgs a) {
             if constexpr (decltype(careful)::value) y = O::finite(y);
             acc[mt] = O::mma32(y, f[j], acc[mt]);
           }
-        if constexpr (O::ES == 2) reads_ahead<2 * D / 32, 4, 2>();
       };
       add(dv, gt, pf);
       add(dk, qt, df);
@@ -757,10 +737,6 @@ void by_block_kv(SArgs a) {
     a.kvodd[(int64_t)bh * a.nblk + desc.blk] = 1;
     walk(std::true_type{});
   }
-  if constexpr (DS) {
-    __syncthreads();
-    put_ds((rows - 1) / NR * NR);
-  }
   // the row groups of a key, through LDS (a [32 keys][D] tile of floats for each key group), then to the item
   float* out = a.kvpart + item * 2 * KT * p.D;
 #pragma unroll
@@ -768,26 +744,21 @@ void by_block_kv(SArgs a) {
     f32x16(&acc)[D / 32] = w ? dv : dk;
     const float sc = w ? 1.f : p.scale;
     if constexpr (RG == 2) {
-      static_assert(2 * 32 * D * 4 <= sizeof(lds) || O::ES == 2);
-      // halves of the columns at a time where the tiles are of 16-bit values
-      constexpr int H = 2 * 32 * D * 4 <= 2 * NR * T::RB ? 1 : 2, MT = D / 32 / H;
+      static_assert(2 * 32 * D * 4 <= sizeof(lds));
+      __syncthreads();
+      float* f = (float*)lds + kg * 32 * D;
+      if (rg == 1) {
 #pragma unroll
-      for (int part = 0; part < H; ++part) {
-        __syncthreads();
-        float* f = (float*)lds + kg * 32 * MT * 32;
-        if (rg == 1) {
+        for (int mt = 0; mt < D / 32; ++mt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int i = 0; i < 16; ++i) f[(mt * 16 + i) * 64 + lane] = acc[mt][i];
+      }
+      __syncthreads();
+      if (rg == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[(mt * 16 + i) * 64 + lane] = acc[part * MT + mt][i];
-        }
-        __syncthreads();
-        if (rg == 0) {
+        for (int mt = 0; mt < D / 32; ++mt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[part * MT + mt][i] += f[(mt * 16 + i) * 64 + lane];
-        }
+          for (int i = 0; i < 16; ++i) acc[mt][i] += f[(mt * 16 + i) * 64 + lane];
       }
       if (rg == 0) put_row<D>(out + ((int64_t)w * KT + key) * p.D, acc, sc, hi, p.D);
     } else {
@@ -797,10 +768,12 @@ void by_block_kv(SArgs a) {
 }
 
 // The same for 16-bit inputs: eight waves, 64 keys, 128 rows at a time.  A wave forms P and dS
-// of 32 rows and 32 keys (its keys' operands in registers) and leaves them in LDS as the
-// operands of the second products, of which each wave takes 32 columns of dV or dK: the sums
-// of a wave are 32 registers where by_block_kv's are 128, so that two waves fit a SIMD and one
-// waits while the other works.
+// of 32 rows and 32 keys and leaves them in LDS as the operands of the second products, of
+// which each wave takes 32 columns of dV or dK: the sums of a wave are 32 registers where
+// by_block_kv's are 128, so that two waves fit a SIMD and one works while the other waits.  DS:
+// dS also goes to memory, rows of block_size keys in the order of the list.  Measured as whole
+// steps against by_block_kv's layout in 16 bits: [1, 8192, 32/8, 128], 16 blocks of 64, 1.75 ->
+// 1.68 ms; 3 of 512, 1.93 -> 1.86 ms; d = 64, 1.19 -> 1.13 ms.
 template <class Tag, int D, bool DS>
 __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2)))
 void by_block_kv16(SArgs a) {
@@ -1728,7 +1701,7 @@ void by_query(SArgs a, int splits, int hgroups) {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-int key_tile(const mattn_selected* p) { return p->block_size >= 128 ? 128 : 64; }
+int key_tile(const mattn_selected* p) { return p->block_size >= 128 && p->dtype == MATTN_F32 ? 128 : 64; }
 
 int sel_check(const mattn_selected* p) {
   if (!p) return MATTN_ERR_NULL;
@@ -2020,24 +1993,16 @@ extern "C" int mattn_selected_bwd(const mattn_selected* p, const void* q, const 
     with_dim(p->D, [&](auto dim) {
       constexpr int D = decltype(dim)::value;
       if (!s.tile_bwd) hipLaunchKernelGGL((by_block_q<Tag, D, true>), dim3((uint32_t)(a.bh_n * l.max_tiles)), dim3(256), 0, st, a);
-      const auto kv = [&](auto kt, auto ds) {
-        if constexpr (decltype(kt)::value == 64 && !std::is_same_v<Tag, float>) {
-          hipLaunchKernelGGL((by_block_kv16<Tag, D, decltype(ds)::value>), dim3((uint32_t)(a.bh_n * l.max_kv)), dim3(512), 0, st, a);
-          return;
-        }
-        hipLaunchKernelGGL((by_block_kv<Tag, D, decltype(kt)::value, decltype(ds)::value>), dim3((uint32_t)(a.bh_n * l.max_kv)),
-                           dim3(256), 0, st, a);
-      };
-      using K64 = std::integral_constant<int, 64>;
-      using K128 = std::integral_constant<int, 128>;
-      if constexpr (!std::is_same_v<Tag, float>) {
-        if (s.tile_bwd) {
-          KT == 128 ? kv(K128{}, std::true_type{}) : kv(K64{}, std::true_type{});
-          hipLaunchKernelGGL((by_tile<Tag, D, true>), tiles, dim3(256), 0, st, a, hg32, tiles_q);
-          return;
-        }
+      const dim3 items((uint32_t)(a.bh_n * l.max_kv));
+      if constexpr (std::is_same_v<Tag, float>) {
+        if (KT == 128) hipLaunchKernelGGL((by_block_kv<D, 128>), items, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((by_block_kv<D, 64>), items, dim3(256), 0, st, a);
+      } else if (s.tile_bwd) {
+        hipLaunchKernelGGL((by_block_kv16<Tag, D, true>), items, dim3(512), 0, st, a);
+        hipLaunchKernelGGL((by_tile<Tag, D, true>), tiles, dim3(256), 0, st, a, hg32, tiles_q);
+      } else {
+        hipLaunchKernelGGL((by_block_kv16<Tag, D, false>), items, dim3(512), 0, st, a);
       }
-      KT == 128 ? kv(K128{}, std::false_type{}) : kv(K64{}, std::false_type{});
     });
     if (!s.tile_bwd) hipLaunchKernelGGL((join_rows<Tag, true>), join, dim3(256), 0, st, a, ll, p->count, false);
     hipLaunchKernelGGL((join_keys<Tag>), keys, dim3(256), 0, st, a, KT);
