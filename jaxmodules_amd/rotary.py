@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -67,6 +68,11 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str
     return f.to(device), scale
 
 
+# mattn_rotary as one record: sizes and types, eps and scale, strides, pointers
+_RECORD = struct.Struct("=12i2f20q10Q")
+assert _RECORD.size == ctypes.sizeof(_lib.MattnRotary)
+
+
 class _Call:
     """One call's tensors and options, as mattn_rotary takes them."""
 
@@ -76,27 +82,24 @@ class _Call:
         self.device = xs[0].device
 
     def record(self, xs, ys, gs=None, inverse=False):
-        B, L, _, D = xs[0].shape
-        p = _lib.MattnRotary(B=B, L=L, D=D, dim=0 if self.inv_freq is None else 2 * self.inv_freq.numel(), n=len(xs),
-                             dtype=DTYPES[xs[0].dtype], layout=self.layout, inverse=inverse, norm=self.norm, eps=self.eps,
-                             scale=self.scale)
-        for t, (x, y) in enumerate(zip(xs, ys)):
-            p.H[t] = x.shape[2]
-            p.x[t], p.y[t] = x.data_ptr(), y.data_ptr()
-            p.x_stride[t][:] = x.stride()[:3]
-            p.y_stride[t][:] = y.stride()[:3]
-            if gs is not None:
-                p.g[t] = gs[t].data_ptr()
-                p.g_stride[t][:] = gs[t].stride()[:3]
-            if self.norm and self.weights[t] is not None:
-                p.w[t] = self.weights[t].data_ptr()
-        if self.positions is not None:
-            p.positions = self.positions.data_ptr()
-            p.pos_bytes = self.positions.element_size()
-            p.pos_stride[:] = self.positions.stride() if self.positions.dim() == 2 else (0, self.positions.stride(0))
-        if self.inv_freq is not None:
-            p.inv_freq = self.inv_freq.data_ptr()
-        return p
+        B, L, H, D = xs[0].shape
+        two = len(xs) == 2
+        dense = (0, 0, 0)
+
+        def strides(ts):
+            return (*ts[0].stride()[:3], *(ts[1].stride()[:3] if two else dense)) if ts else (*dense, *dense)
+
+        def pointers(ts):
+            return (ts[0].data_ptr(), ts[1].data_ptr() if two else 0) if ts else (0, 0)
+
+        pos, f = self.positions, self.inv_freq
+        w = [0 if x is None else x.data_ptr() for x in self.weights] if self.norm else [0, 0]
+        return _lib.MattnRotary.from_buffer_copy(_RECORD.pack(
+            B, L, D, 0 if f is None else 2 * f.numel(), len(xs), H, xs[1].shape[2] if two else 0, DTYPES[xs[0].dtype],
+            self.layout, inverse, self.norm, 0 if pos is None else pos.element_size(), self.eps, self.scale,
+            *((0, 0) if pos is None else pos.stride() if pos.dim() == 2 else (0, pos.stride(0))),
+            *strides(xs), *strides(ys), *strides(gs), *pointers(xs), *pointers(ys), *pointers(gs),
+            w[0], w[1] if two else 0, 0 if pos is None else pos.data_ptr(), 0 if f is None else f.data_ptr()))
 
     def forward(self, xs, inverse=False):
         ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
@@ -179,8 +182,8 @@ def _rotate(name, q, k, weights, positions, inv_freq, layout, scale, norm, eps):
         raise NotImplementedError(f"{name}: head dimension {D} is not supported (1 to {MAX_D})")
     if layout not in LAYOUTS:
         raise ValueError(f"{name}: layout must be 'half' or 'interleaved', got {layout!r}")
-    if not math.isfinite(scale):
-        raise ValueError(f"{name}: scale must be finite, got {scale}")
+    if not abs(scale) < 3.4028235677973366e38:
+        raise ValueError(f"{name}: scale must be a finite float32, got {scale}")
     if inv_freq is None:
         if not norm:
             raise ValueError(f"{name} needs inv_freq")
@@ -198,8 +201,8 @@ def _rotate(name, q, k, weights, positions, inv_freq, layout, scale, norm, eps):
     for w in given:
         if w.shape != (D,) or w.dtype not in DTYPES:
             raise ValueError(f"{name}: weights must be [{D}] of a floating dtype, got {w.dtype} {tuple(w.shape)}")
-    if norm and not (math.isfinite(eps) and eps >= 0):
-        raise ValueError(f"{name}: eps must be finite and not negative, got {eps}")
+    if norm and not 0 <= eps < 3.4028235677973366e38:
+        raise ValueError(f"{name}: eps must be a finite float32 and not negative, got {eps}")
     on_gpu(name, *xs, positions, inv_freq, *given)
     xs = [rows(x) for x in xs]
     w32 = [None if w is None else w.detach().float().contiguous() for w in weights[: len(xs)]] if norm else None

@@ -20,7 +20,9 @@ head h // (Hq / Hkv).  There is no CPU code path.
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -167,6 +169,11 @@ def _scratch(nbytes, device):
     return ws, ptr, nbytes
 
 
+# mattn_selected as one record: sizes and types, scale, 8 x 3 strides, pointers
+_RECORD = struct.Struct("=10if4x24q3Q")
+assert _RECORD.size == ctypes.sizeof(_lib.MattnSelected)
+
+
 class _Call:
     """What a call of the attention is besides its tensors of values."""
 
@@ -176,14 +183,10 @@ class _Call:
 
     def record(self, q, k, v, o, do=None, dq=None, dk=None, dv=None):
         B, N, Hq, d = q.shape
-        p = _lib.MattnSelected(B=B, Lq=N, Lk=k.shape[1], Hq=Hq, Hkv=k.shape[2], D=d, dtype=DTYPES[q.dtype],
-                               block_size=self.block_size, count=self.blocks.shape[3], causal=self.causal,
-                               scale=self.scale, blocks=self.blocks.data_ptr(), starts=_ptr(self.starts),
-                               lengths=_ptr(self.lengths))
-        for f, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", do), ("dq", dq), ("dk", dk), ("dv", dv)):
-            if t is not None:
-                getattr(p, f + "_stride")[:] = t.stride()[:3]
-        return p
+        strides = [(0, 0, 0) if t is None else t.stride()[:3] for t in (q, k, v, o, do, dq, dk, dv)]
+        return _lib.MattnSelected.from_buffer_copy(_RECORD.pack(
+            B, N, k.shape[1], Hq, k.shape[2], d, DTYPES[q.dtype], self.block_size, self.blocks.shape[3], self.causal,
+            self.scale, *itertools.chain(*strides), self.blocks.data_ptr(), _ptr(self.starts) or 0, _ptr(self.lengths) or 0))
 
     def forward(self, q, k, v, grads):
         """(O, what the backward keeps: float32 O, lse and the blocks' lists)."""
