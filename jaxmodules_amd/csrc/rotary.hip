@@ -22,10 +22,10 @@
 // Waiting for a row before asking for the next left half the bandwidth unused: a lane now
 // asks for its next head's row before it works on the one at hand.  The backward gives
 // each tensor its own workgroups, whose weight gradients then fit the registers (both
-// tensors' spilled: 148 us against 121).  Measured, bf16, 32 + 8 heads of 128: 16384
-// positions forward 63 us (5.3 TB/s); 2 x 4096 forward with its gradient 51 + 121 + 7 us
-// for 671 MB (3.7 TB/s; a copy of that size reaches 4.8 TB/s).  A one-token call is 5 us
-// of kernel.
+// tensors' spilled: 148 us against 121).  Measured, bf16, d = 128: 16384 positions of 32 + 8
+// heads forward 63 us (5.3 TB/s); 8192 of 32 + 32 heads forward 51 us (5.3 TB/s), backward
+// 121 us (3.3 TB/s; a copy reaches 4.8 TB/s) and 7 us of weights.  A one-token call is 5 us of
+// kernel.
 #include "elem.hpp"
 
 namespace mattn {

@@ -441,16 +441,22 @@ void by_block_q(SArgs a) {
     if (odd) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
   };
 
+  constexpr bool EARLY = O::ES == 2 || !GRAD || D == 64;  // (float32's Q and dO at D = 128: 128 registers, twice would spill)
   Rows next;
-  load(next, 0);
+  if constexpr (EARLY) load(next, 0);
   if constexpr (AHEAD) fetch(0);
   int buf = 0;
   bool odd = false;  // GRAD: some tile of K holds an infinite or NaN value
   for (int r0 = 0; r0 < rows; r0 += 128) {
     const bool live = r0 + 32 * wave + l32 < rows;
-    Rows now = next;
+    Rows now;
+    if constexpr (EARLY) {
+      now = next;
+      if (r0 + 128 < rows) load(next, r0 + 128);
+    } else {
+      load(now, r0);
+    }
     const RowId id = now.id;
-    if (r0 + 128 < rows) load(next, r0 + 128);
     const int64_t row = ((int64_t)bh * p.Lq + id.q) * a.G + id.g;
     const int64_t lim = key_limit(p, b, id.q, held, start) - k0;  // keys of the block the row sees
     const int seen = (int)min(lim, (int64_t)inside);
@@ -503,6 +509,10 @@ void by_block_q(SArgs a) {
             if (ko) a.odd[(int64_t)bh * a.nblk + desc.blk] = 1;
             odd = __syncthreads_or(ko) || odd;
           }
+          // (opaque: places in LDS worked out ahead of the loop would take the registers of the operands)
+          int tid = threadIdx.x;
+          asm("" : "+v"(tid));
+          const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
           const bool part = __any(seen < (t + 1) * kKT);  // some row of the wave does not see all of the tile
           // S^T of 32 keys, single floats from here on (as in attend_tile)
           const auto scores = [&](const char* tile, const typename O::Frag(&f)[D / 16], int x, float(&s)[16]) {
